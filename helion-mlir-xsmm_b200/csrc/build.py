@@ -31,9 +31,12 @@ SOURCES = [
     "gemm_umma.cu",
     "host_rows.cu",
     "attention.cu",
+    "attention_packed.cu",
+    "kv_cache.cu",
+    "attention_cached.cu",
     "peer.cu",
 ]
-HEADERS = ["common.cuh", "gemm_common.cuh", "umma_ptx.cuh", "../../include/b200ops.h"]
+HEADERS = ["common.cuh", "gemm_common.cuh", "umma_ptx.cuh", "sequences.cuh", "kv_cache.cuh", "../../include/b200ops.h"]
 FLAGS = [
     "-gencode",
     "arch=compute_100a,code=sm_100a",

@@ -128,6 +128,51 @@ class PeerOut(ctypes.Structure):
     ]
 
 
+class PackedAttentionDesc(ctypes.Structure):
+    """``b200_packed_attention_desc`` of include/b200ops.h."""
+
+    _fields_ = [
+        ("dtype", c_int32),
+        ("causal", c_int32),
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("q_row", c_int64),
+        ("q_head", c_int64),
+        ("k_row", c_int64),
+        ("k_head", c_int64),
+        ("v_row", c_int64),
+        ("v_head", c_int64),
+        ("rows_q", c_int64),
+        ("rows_k", c_int64),
+        ("batch", c_int64),
+        ("heads", c_int64),
+        ("kv_heads", c_int64),
+        ("dim", c_int64),
+        ("offsets", c_void_p),
+        ("k_offsets", c_void_p),
+        ("scale", c_float),
+        ("reserved_", c_int32),
+    ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """``b200_kv_cache`` of include/b200ops.h."""
+
+    _fields_ = [
+        ("k_codes", c_void_p),
+        ("v_codes", c_void_p),
+        ("k_scales", c_void_p),
+        ("v_scales", c_void_p),
+        ("blocks", c_int64),
+        ("heads", c_int32),
+        ("dim", c_int32),
+        ("block_tokens", c_int32),
+        ("reserved_", c_int32),
+    ]
+
+
 class Counters(ctypes.Structure):
     _fields_ = [
         ("launches", c_uint64),
@@ -149,6 +194,24 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "b200_attention": (
         c_int,
         [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p],
+    ),
+    "b200_attention_packed": (c_int, [ctypes.POINTER(PackedAttentionDesc), c_void_p]),
+    "b200_kv_append": (
+        c_int,
+        [ctypes.POINTER(KvCacheDesc), c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
+         c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p],
+    ),
+    "b200_kv_read": (
+        c_int,
+        [ctypes.POINTER(KvCacheDesc), c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+         c_int64, c_int64, c_void_p],
+    ),
+    "b200_attention_cached_workspace_bytes": (
+        c_size_t, [ctypes.POINTER(KvCacheDesc), c_int64, c_int64, c_int64, c_int64]),
+    "b200_attention_cached": (
+        c_int,
+        [ctypes.POINTER(KvCacheDesc), c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+         c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p, c_size_t, c_void_p],
     ),
     "b200_pack": (
         c_int,

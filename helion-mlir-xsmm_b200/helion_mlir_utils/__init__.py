@@ -1,14 +1,16 @@
 """The helion_mlir_utils operator set, B200-native.
 
 The 30 names of the reference's ``helion_mlir_utils/__init__.py`` with the same
-signatures, plus ``layer_norm``, ``rms_norm``, ``matmul_blocked`` and the fused
-epilogue helpers. Every operator enqueues hand-written sm_100a kernels from
+signatures, plus ``layer_norm``, ``rms_norm``, ``matmul_blocked``, the fused
+epilogue helpers, and what serving a language model needs beside them: attention over
+packed prompts and over a key/value cache in 8 bits. Every operator enqueues hand-written sm_100a kernels from
 ``libb200ops.so`` on the caller's current CUDA stream.
 """
 
 from __future__ import annotations
 
 from .attention import attention
+from .attention import attention_packed
 from .elementwise import leaky_relu
 from .elementwise import relu
 from .elementwise import scalar_mul
@@ -16,6 +18,11 @@ from .host_io import stream_rows
 from .epilogues import gelu_tanh
 from .epilogues import leaky_relu_epilogue
 from .kernels import per_config
+from .kv_cache import QuantizedCache
+from .kv_cache import attention_cached
+from .kv_cache import cache_append
+from .kv_cache import cache_read
+from .kv_cache import quantized_cache
 from .linear import CACHE_PREPACKED_WEIGHTS_ENV
 from .linear import AffineLinearCache
 from .linear import LinearCache
@@ -65,10 +72,15 @@ __all__ = [
     "CACHE_PREPACKED_WEIGHTS_ENV",
     "AffineLinearCache",
     "LinearCache",
+    "QuantizedCache",
     "add_extra",
     "attention",
+    "attention_cached",
+    "attention_packed",
     "bmm",
+    "cache_append",
     "cache_prepacked_weights",
+    "cache_read",
     "column_sharded_linear",
     "column_sum",
     "gather_rows",
@@ -97,6 +109,7 @@ __all__ = [
     "pad_2d",
     "per_config",
     "prepacked_b_call",
+    "quantized_cache",
     "relu",
     "rms_norm",
     "row_dot",
@@ -119,7 +132,7 @@ __all__ = [
 # HELION_MLIR_TRACE_CALLS=1: every operator reports the first call with each kind of
 # operands and an at-exit summary counts the calls. Unset: nothing is wrapped.
 _OPERATORS = [
-    "attention", "bmm", "column_sum", "group_norm", "layer_norm", "leaky_relu", "linear", "linear_affine", "matmul",
+    "attention", "attention_cached", "attention_packed", "bmm", "cache_append", "cache_read", "column_sum", "group_norm", "layer_norm", "leaky_relu", "linear", "linear_affine", "matmul",
     "matmul_blocked", "matmul_host", "matmul_prepacked_b", "matmul_prepacked_b_affine", "matvec", "pack_a_blocked",
     "pack_a_blocked_t", "pack_b_blocked", "pack_b_blocked_t", "pack_b_blocked_vnni", "pack_b_blocked_vnni_t",
     "pack_b_vnni_t", "pad_2d", "relu", "rms_norm", "row_dot", "row_sum", "scalar_mul", "softmax", "stream_rows",

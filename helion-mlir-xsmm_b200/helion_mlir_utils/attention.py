@@ -9,10 +9,14 @@ tensor-core kernel ``b200_attention`` (scores and probabilities never leave the
 SM). Everything else (f32, other head sizes) is composed from the operators of
 this package: one batched GEMM for the scores, the row softmax, one batched GEMM
 with ``v`` -- the scores then pass through HBM once in f32.
+
+``attention_packed`` is the form that prompts need: sequences of different lengths packed
+into one tensor, causal, several query heads to a key/value head.
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -20,6 +24,7 @@ from torch import Tensor
 
 from helion_mlir_backend import native
 from helion_mlir_backend import output_pool
+from helion_mlir_backend.call_trace import CallExplanation
 from helion_mlir_backend.call_trace import trace
 
 _FUSED_DIMS = (64, 128)
@@ -86,3 +91,70 @@ def explain_attention(q: Tensor, k: Tensor, v: Tensor, scale: float | None = Non
 
 
 attention.explain = explain_attention  # type: ignore[attr-defined]
+
+
+# ------------------------------------------------------------------------------- packed sequences
+
+_MAX_DIM = 256
+
+
+def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor) -> None:
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"attention_packed() expects [rows, heads, dim] operands, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape != v.shape or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("attention_packed() operands do not match (the heads of q have to be a multiple of those of k and v): "
+                         f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if not 1 <= q.shape[2] <= _MAX_DIM:
+        raise ValueError(f"attention_packed() expects heads of 1 to {_MAX_DIM}, got {tuple(q.shape)}")
+    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"attention_packed() requires matching bf16/f32 operands, got {q.dtype}, {k.dtype}, {v.dtype}")
+    for name, t in (("offsets", offsets), ("k_offsets", k_offsets)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape != offsets.shape or t.shape[0] < 1 or not t.is_contiguous():
+            raise ValueError(f"attention_packed() expects {name} as a contiguous int32 tensor [sequences + 1], got {t.dtype} {tuple(t.shape)}")
+    if k_offsets is offsets and k.shape[0] != q.shape[0]:
+        raise ValueError(f"attention_packed() needs k_offsets where k has other rows than q: {tuple(q.shape)}, {tuple(k.shape)}")
+
+
+def _packed_desc(q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, offsets: Tensor, k_offsets: Tensor, scale: float,
+                 causal: bool) -> native.PackedAttentionDesc:
+    rows, heads, dim = q.shape
+    return native.PackedAttentionDesc(
+        native.dtype_code(q.dtype), causal, q.data_ptr(), k.data_ptr(), v.data_ptr(), native.ptr(out), q.stride(0), q.stride(1),
+        k.stride(0), k.stride(1), v.stride(0), v.stride(1), rows, k.shape[0], offsets.shape[0] - 1, heads, k.shape[1], dim,
+        offsets.data_ptr(), k_offsets.data_ptr(), scale, 0)
+
+
+def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor | None = None,
+                     scale: float | None = None, causal: bool = True) -> Tensor:
+    """Attention of packed sequences: ``softmax(scale * q @ k^T) @ v`` of each sequence's queries over its own keys.
+
+    ``q``: ``[rows, heads, dim]``, ``k``, ``v``: ``[key rows, kv_heads, dim]``, bf16 or f32, ``dim`` up to 256; views with
+    strides (slices of a fused projection) are read in place. Query head ``h`` reads key/value head
+    ``h // (heads // kv_heads)``. ``offsets``, ``k_offsets`` (int32 on the device, ``[sequences + 1]``): sequence ``b`` owns the
+    rows ``offsets[b] .. offsets[b + 1]``; ``k_offsets`` defaults to ``offsets`` (a prompt over itself) and differs where a part of
+    the keys was computed before. ``causal``: the queries are the last positions of the keys, row ``i`` of ``n`` sees
+    key ``j`` of ``m`` if ``j <= i + m - n``. A row that sees no key is zeros, and so are rows behind the last
+    sequence. What a row does not see does not reach it, infinities and NaN included. ``scale`` defaults to ``dim ** -0.5``.
+
+    The offsets are not read on the host: a captured call can be replayed with other lengths of the same total. Offsets
+    that decrease or leave the tensors raise bit 256 of ``native.kernel_status()`` and leave their rows unwritten."""
+    k_offsets = offsets if k_offsets is None else k_offsets
+    _check_packed(q, k, v, offsets, k_offsets)
+    device = native.require_cuda(q, k, v, offsets, k_offsets)
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
+    with native.on_device(device):
+        out = output_pool.empty(tuple(q.shape), dtype=q.dtype, device=device)
+        desc = _packed_desc(q, k, v, out, offsets, k_offsets, scale, bool(causal))
+        code = native.module().b200_attention_packed(ctypes.byref(desc), native.stream_ptr(device))
+    native.check("b200_attention_packed", code)
+    return out
+
+
+def _explain_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor | None = None,
+                    scale: float | None = None, causal: bool = True) -> CallExplanation:
+    _check_packed(q, k, v, offsets, offsets if k_offsets is None else k_offsets)
+    return CallExplanation(True, "packed_simt_kernel (f32 tiles of 64 x 64)")
+
+
+attention_packed.explain = _explain_packed  # type: ignore[attr-defined]

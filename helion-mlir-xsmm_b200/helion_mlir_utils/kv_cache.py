@@ -1,0 +1,212 @@
+"""A key/value cache held in 8 bits and the attention that reads it (no counterpart in the
+reference, which has attention over whole operands only).
+
+The cache is four tensors, a :class:`QuantizedCache` or any tuple of the same four:
+
+* ``k_codes`` int8 ``[blocks, heads, tokens, dim]`` and ``v_codes`` int8 ``[blocks, heads, dim, tokens]``
+  (V's tokens side by side: the product with the probabilities sums over them);
+* ``k_scales``, ``v_scales`` f32 ``[blocks, heads]``: a value is ``code * scale``.
+
+A block holds 16, 32 or 64 tokens; ``dim`` is 64 or 128. Position ``p`` of sequence ``b`` lies in block
+``block_table[b, p // tokens]``; who owns which block is the caller's business. Lengths, starts, offsets and the
+table are int32 tensors on the device: no call reads them on the host, so all of them can be captured into a CUDA
+graph and replayed with other contents. Block numbers outside the cache and positions beyond the table
+are not followed: they raise bit 512 of ``native.kernel_status()``, writes skip them and what
+reads them answers NaN.
+
+A serving loop: :func:`~helion_mlir_utils.attention_packed` over the prompts and :func:`cache_append` of their keys and
+values, then for each token :func:`cache_append` and :func:`attention_cached`; :func:`cache_read` gives a cached
+prefix back for ``attention_packed`` of a later chunk of the prompt.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from helion_mlir_backend import native
+from helion_mlir_backend import output_pool
+from helion_mlir_backend.call_trace import CallExplanation
+
+BLOCK_TOKENS = (16, 32, 64)
+HEAD_DIMS = (64, 128)
+
+
+class QuantizedCache(NamedTuple):
+    """Codes and scales of an 8-bit key/value cache; :func:`quantized_cache` allocates one."""
+
+    k_codes: Tensor
+    v_codes: Tensor
+    k_scales: Tensor
+    v_scales: Tensor
+
+
+def quantized_cache(blocks: int, heads: int, dim: int, block_tokens: int = 64, device: torch.device | str = "cuda") -> QuantizedCache:
+    """An empty cache of ``blocks`` blocks for ``heads`` key/value heads. Each head costs ``2 * dim`` bytes a token
+    and 8 bytes a block."""
+    if blocks < 0 or heads < 1 or dim not in HEAD_DIMS or block_tokens not in BLOCK_TOKENS:
+        raise ValueError(f"quantized_cache() expects heads >= 1, dim in {HEAD_DIMS} and block_tokens in {BLOCK_TOKENS}, "
+                         f"got {blocks} blocks, heads {heads}, dim {dim}, block_tokens {block_tokens}")
+    return QuantizedCache(
+        torch.zeros(blocks, heads, block_tokens, dim, dtype=torch.int8, device=device),
+        torch.zeros(blocks, heads, dim, block_tokens, dtype=torch.int8, device=device),
+        torch.zeros(blocks, heads, dtype=torch.float32, device=device),
+        torch.zeros(blocks, heads, dtype=torch.float32, device=device),
+    )
+
+
+def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[native.KvCacheDesc, int, int]:
+    """The library's view of the cache, its heads and head size."""
+    k_codes, v_codes, k_scales, v_scales = cache
+    if k_codes.dim() != 4 or v_codes.dim() != 4:
+        raise ValueError(f"{name}() expects codes [blocks, heads, tokens, dim] and [blocks, heads, dim, tokens], "
+                         f"got {tuple(k_codes.shape)} and {tuple(v_codes.shape)}")
+    blocks, heads, tokens, dim = k_codes.shape
+    if dim not in HEAD_DIMS or tokens not in BLOCK_TOKENS or heads < 1:
+        raise ValueError(f"{name}() expects blocks of {BLOCK_TOKENS} tokens and heads of {HEAD_DIMS}, got codes {tuple(k_codes.shape)}")
+    if v_codes.shape != (blocks, heads, dim, tokens) or k_scales.shape != (blocks, heads) or v_scales.shape != (blocks, heads):
+        raise ValueError(f"{name}() cache tensors do not match: codes {tuple(k_codes.shape)} and {tuple(v_codes.shape)}, "
+                         f"scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}")
+    if (k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or k_scales.dtype != torch.float32
+            or v_scales.dtype != torch.float32):
+        raise ValueError(f"{name}() expects int8 codes and f32 scales, got {k_codes.dtype}, {v_codes.dtype}, {k_scales.dtype}, {v_scales.dtype}")
+    if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
+        raise ValueError(f"{name}() expects contiguous cache tensors")
+    return native.KvCacheDesc(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), blocks, heads,
+                              dim, tokens, 0), heads, dim
+
+
+def _indices(name: str, what: str, t: Tensor, shape: tuple[int, ...]) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}() expects {what} as a contiguous int32 tensor {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _table(name: str, table: Tensor) -> tuple[int, int, int]:
+    """Sequences, row stride and width of a block table."""
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{name}() expects block_table as an int32 tensor [sequences, blocks] with contiguous rows, "
+                         f"got {table.dtype} {tuple(table.shape)}")
+    batch, width = table.shape
+    return batch, max(table.stride(0), width), width
+
+
+def _aligned_rows(t: Tensor) -> Tensor:
+    """``t`` if its rows can be read as 16-byte vectors, else a contiguous copy."""
+    step = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def cache_append(cache: tuple[Tensor, Tensor, Tensor, Tensor], k: Tensor, v: Tensor, block_table: Tensor, lengths: Tensor,
+                 offsets: Tensor | None = None) -> None:
+    """Write new keys and values behind the ``lengths[b]`` positions that sequence ``b`` holds, in place.
+
+    ``k``, ``v``: bf16 or f32, ``[rows, heads, dim]`` with sequence ``b`` owning the rows ``offsets[b] .. offsets[b + 1]``
+    (int32, ``[sequences + 1]``); without ``offsets``, ``[sequences, heads, dim]`` (one token each) or
+    ``[sequences, new, heads, dim]``. Views with strides (slices of a fused projection) are read in place.
+
+    Scale of a block and head: ``max(max|x| / 127, 2^-100)`` over the block's tokens; it grows while the block fills and never
+    shrinks, and when it grows the older codes become ``rint(code * old / new)``. Codes are rounded to the nearest, ties to
+    even. A value that is not finite makes the scale NaN. ``lengths`` is left as it is (the caller adds the
+    new tokens); the blocks have to be in the table already. No block may belong to two of the sequences that are written."""
+    desc, heads, dim = _describe(cache, "cache_append")
+    batch, stride, width = _table("cache_append", block_table)
+    if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"cache_append() expects matching bf16/f32 k and v, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    if tuple(k.shape[-2:]) != (heads, dim) or k.dim() not in ((3,) if offsets is not None else (3, 4)):
+        raise ValueError(f"cache_append() expects k and v [rows, {heads}, {dim}] (or [sequences, new, {heads}, {dim}] without "
+                         f"offsets), got {tuple(k.shape)}")
+    _indices("cache_append", "lengths", lengths, (batch,))
+    if offsets is not None:
+        _indices("cache_append", "offsets", offsets, (batch + 1,))
+    elif k.shape[0] != batch:
+        raise ValueError(f"cache_append() expects k and v of {batch} sequences, got {tuple(k.shape)}")
+    device = native.require_cuda(*cache, k, v, block_table, lengths, offsets)
+    if k.dim() == 4:
+        k, v = k.flatten(0, 1), v.flatten(0, 1)
+    k, v = _aligned_rows(k), _aligned_rows(v)
+    with native.on_device(device):
+        code = native.module().b200_kv_append(
+            ctypes.byref(desc), native.dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
+            v.stride(1), block_table.data_ptr(), stride, width, lengths.data_ptr(), native.ptr(offsets), batch, k.shape[0],
+            native.stream_ptr(device),
+        )
+    native.check("b200_kv_append", code)
+
+
+def cache_read(cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, starts: Tensor, lengths: Tensor,
+               offsets: Tensor, rows: int, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
+    """Positions ``starts[b] ...`` of each sequence as values: ``(k, v)``, each ``[rows, heads, dim]`` in ``dtype`` (bf16 or f32),
+    packed: sequence ``b`` fills the rows ``offsets[b] .. offsets[b + 1]``. Positions that the sequence does not
+    hold (at or beyond ``lengths[b]``) and rows behind the last sequence are zeros."""
+    desc, heads, dim = _describe(cache, "cache_read")
+    batch, stride, width = _table("cache_read", block_table)
+    if dtype not in (torch.bfloat16, torch.float32) or rows < 0:
+        raise ValueError(f"cache_read() expects rows >= 0 and dtype bf16/f32, got {rows} and {dtype}")
+    _indices("cache_read", "starts", starts, (batch,))
+    _indices("cache_read", "lengths", lengths, (batch,))
+    _indices("cache_read", "offsets", offsets, (batch + 1,))
+    device = native.require_cuda(*cache, block_table, starts, lengths, offsets)
+    with native.on_device(device):
+        k = output_pool.empty((rows, heads, dim), dtype=dtype, device=device)
+        v = output_pool.empty((rows, heads, dim), dtype=dtype, device=device)
+        code = native.module().b200_kv_read(
+            ctypes.byref(desc), native.dtype_code(dtype), k.data_ptr(), v.data_ptr(), block_table.data_ptr(), stride, width,
+            starts.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), batch, rows, native.stream_ptr(device),
+        )
+    native.check("b200_kv_read", code)
+    return k, v
+
+
+def _check_cached(q: Tensor, heads: int, dim: int, batch: int) -> None:
+    if q.dtype not in (torch.bfloat16, torch.float32) or q.dim() not in (3, 4) or q.shape[-1] != dim or q.shape[-2] % heads:
+        raise ValueError(f"attention_cached() expects bf16/f32 q [sequences, heads, {dim}] or [sequences, tokens, heads, {dim}] with "
+                         f"heads a multiple of {heads}, got {q.dtype} {tuple(q.shape)}")
+    if q.shape[0] != batch or q.shape[-2] == 0:
+        raise ValueError(f"attention_cached() expects q of {batch} sequences and at least one head, got {tuple(q.shape)}")
+
+
+def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, lengths: Tensor,
+                     scale: float | None = None) -> Tensor:
+    """``softmax(scale * q @ k^T) @ v`` over the cached positions; ``scale`` defaults to ``dim ** -0.5``.
+
+    ``q``: bf16 or f32, ``[sequences, heads, dim]`` (one token each) or ``[sequences, tokens, heads, dim]``: the last
+    ``tokens`` of the ``lengths[b]`` positions of sequence ``b``, which :func:`cache_append` has written already;
+    token ``i`` sees the positions below ``lengths[b] - tokens + i + 1`` (a row that sees none is zeros). Query head ``h`` reads
+    key/value head ``h // (heads // kv_heads)``. Result in ``q``'s type and shape."""
+    desc, heads, dim = _describe(cache, "attention_cached")
+    batch, stride, width = _table("attention_cached", block_table)
+    _check_cached(q, heads, dim, batch)
+    _indices("attention_cached", "lengths", lengths, (batch,))
+    device = native.require_cuda(q, *cache, block_table, lengths)
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    tokens = 1 if q.dim() == 3 else q.shape[1]
+    lib = native.module()
+    with native.on_device(device):
+        out = output_pool.empty(tuple(q.shape), dtype=q.dtype, device=device)
+        need = lib.b200_attention_cached_workspace_bytes(ctypes.byref(desc), batch, tokens, q.shape[-2], width)
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        code = lib.b200_attention_cached(
+            ctypes.byref(desc), native.dtype_code(q.dtype), q.data_ptr(), q.stride(0), q.stride(1) if tokens > 1 else 0,
+            q.stride(-2), out.data_ptr(), block_table.data_ptr(), stride, width, lengths.data_ptr(), batch, tokens, q.shape[-2],
+            scale, native.ptr(workspace), need, native.stream_ptr(device),
+        )
+    native.check("b200_attention_cached", code)
+    return out
+
+
+def _explain_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, lengths: Tensor,
+                    scale: float | None = None) -> CallExplanation:
+    _, heads, dim = _describe(cache, "attention_cached")
+    _check_cached(q, heads, dim, _table("attention_cached", block_table)[0])
+    return CallExplanation(True, "cached_simple_kernel")
+
+
+attention_cached.explain = _explain_cached  # type: ignore[attr-defined]

@@ -169,6 +169,78 @@ int b200_host_rows_release(void);
 int b200_attention(int32_t dtype, const void* q, const void* k, const void* v, void* out, int64_t heads,
                    int64_t seq_q, int64_t seq_k, int64_t dim, float scale, void* stream);
 
+/* Prompt attention over packed sequences (no counterpart in the reference):
+ * out_i = sum_j softmax_j(scale q_i . k_j) v_j for each query row of a sequence over that
+ * sequence's keys. q: [rows_q][heads][dim], k, v: [rows_k][kv_heads][dim] with any row and
+ * head strides (in elements) and contiguous dim; out: [rows_q][heads][dim] contiguous. Query
+ * head h reads key/value head h / (heads / kv_heads). Sequence b owns the rows
+ * [offsets[b], offsets[b+1]) of q and [k_offsets[b], k_offsets[b+1]) of k and v (device
+ * memory, batch + 1 values each, not decreasing). causal: the queries are the last
+ * positions of the keys: row i of nq sees key j of nk if j <= i + nk - nq. A row that sees no
+ * key is zeros, and so are the rows of out behind the last sequence. Values that a row does
+ * not see never reach it, infinities and NaN included. Sums and the softmax are f32; with bf16
+ * operands the probabilities are rounded to bf16 for the second product. dtype B200_F32 or
+ * B200_BF16, dim 1..256, element-aligned operands. Offsets that decrease or reach outside the
+ * tensors leave their sequence's rows unwritten and OR 256 into the kernel status word. */
+typedef struct b200_packed_attention_desc {
+  int32_t dtype, causal;
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int64_t rows_q, rows_k, batch, heads, kv_heads, dim;
+  const int32_t *offsets, *k_offsets;
+  float scale;
+  int32_t reserved_;
+} b200_packed_attention_desc;
+int b200_attention_packed(const b200_packed_attention_desc* desc, void* stream);
+
+/* A key/value cache in 8 bits (no counterpart in the reference). A block holds
+ * `block_tokens` (16, 32 or 64) positions of every key/value head:
+ *   k_codes [blocks][heads][block_tokens][dim], v_codes [blocks][heads][dim][block_tokens],
+ *   k_scales, v_scales [blocks][heads] f32;  value = code * scale.  dim 64 or 128.
+ * Position p of sequence b lies in block block_table[b * table_stride + p / block_tokens]
+ * (device memory, `table_width` entries a sequence). A block number outside the cache or a
+ * position beyond the table is never followed: it ORs 512 into the kernel status word, a
+ * write skips it, and a read or an attention over it answers NaN. All strides are in elements;
+ * k, v and q keep dim contiguous. */
+typedef struct b200_kv_cache {
+  void *k_codes, *v_codes;
+  float *k_scales, *v_scales;
+  int64_t blocks;
+  int32_t heads, dim, block_tokens, reserved_;
+} b200_kv_cache;
+
+/* Writes new tokens behind the lengths[b] positions that sequence b holds. k, v: `rows` packed rows of
+ * [heads][dim], 16-byte aligned with strides that keep it so; sequence b owns the rows
+ * [offsets[b], offsets[b+1]), or, with offsets == NULL, rows / batch each. For each
+ * touched (block, head) of K and of V: s = max(max|x| / 127, 2^-100, and the old scale if
+ * the block holds older tokens of the sequence); codes are x / s rounded to the nearest,
+ * ties to even; where s grew, older codes become code * s_old / s, rounded the same way. A value
+ * that is not finite makes s NaN (for the rest of the block's use). `lengths` is not changed.
+ * No block may be written for two sequences in one call. */
+int b200_kv_append(const b200_kv_cache* cache, int32_t dtype, const void* k, const void* v, int64_t k_row, int64_t k_head,
+                   int64_t v_row, int64_t v_head, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                   const int32_t* lengths, const int32_t* offsets, int64_t batch, int64_t rows, void* stream);
+
+/* Reads positions starts[b] ... of each sequence back as values: k_out, v_out [rows][heads][dim]
+ * contiguous (16-byte aligned); sequence b fills the rows [offsets[b], offsets[b+1]).
+ * Positions at or beyond lengths[b] and the rows behind the last sequence are zeros. */
+int b200_kv_read(const b200_kv_cache* cache, int32_t dtype, void* k_out, void* v_out, const int32_t* block_table,
+                 int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths,
+                 const int32_t* offsets, int64_t batch, int64_t rows, void* stream);
+
+/* Attention of the last `tokens` positions of each sequence (lengths[b] positions, these
+ * included) over the cache: q [batch][tokens][heads][dim], out the same, contiguous;
+ * token i sees the positions below lengths[b] - tokens + i + 1, none: zeros. Sums and the
+ * softmax are f32. The workspace (16-byte aligned, of the size the query says) holds partial
+ * results during the call; nothing in it has to be kept or cleared. */
+size_t b200_attention_cached_workspace_bytes(const b200_kv_cache* cache, int64_t batch, int64_t tokens, int64_t heads,
+                                             int64_t table_width);
+int b200_attention_cached(const b200_kv_cache* cache, int32_t dtype, const void* q, int64_t q_batch, int64_t q_token,
+                          int64_t q_head, void* out, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                          const int32_t* lengths, int64_t batch, int64_t tokens, int64_t heads, float scale,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 /* Layout conversions (bit-exact copies with zero fill). `kind`: */
 enum {
   B200_PACK_PAD_2D = 0,         /* [r,c] -> [rows_pad, cols_pad]                       matmul.py:78-89 */
