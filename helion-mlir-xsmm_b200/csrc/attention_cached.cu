@@ -3,15 +3,45 @@
 // j <= lengths - tokens + i, k_j = code * k_scale[block, head], v_j = code * v_scale[block, head].
 // q, out: [batch][tokens][heads][dim]; query head h reads key/value head h / group. A row that
 // sees nothing is zeros. No reference counterpart.
+//
+// Bound by HBM: every code is read once, 2 dim bytes a token and key/value head, against
+// 4 dim flops a token and query head. Each warp is a worker of its own: all tiles of 64 positions of all
+// (sequence, key/value head) pairs are numbered in one line, and worker w takes the w-th equal part of it, so
+// ragged lengths leave nobody idle, whatever they are (the host never reads them). A pair that lies
+// in one part is finished there; of the others each worker leaves its maximum, sum and
+// accumulator, which a second kernel joins in a fixed order. Within a warp:
+//   * The codes arrive by bulk copies into the warp's own ring of slots (a tile of K, a tile of V, ...); a slot is
+//     refilled as soon as the warp has read it, so there are no barriers between warps.
+//   * The products run as D = A B with the codes as A and the few query rows as the 8 columns of B
+//     (mma m16n8k16), S^T = K Q^T and O^T = V^T P^T: 8 query rows fill an instruction, with the
+//     queries as A they would fill half of it. tcgen05.mma would take 64 rows at least and its operands
+//     from shared memory, in 16 bits: the codes would be written back there once more.
+//   * A code is exact in f16 (and in bf16, at twice the instructions): one byte permutation puts it into
+//     the mantissa of 1024 + code + 128, one packed subtraction takes 1152 off. The dims
+//     within a product, and the tokens within the second one, are taken in the order in which a thread finds
+//     them in 16 consecutive bytes; P gets into that order by the choice of the token for each row of S^T.
+//   * P carries V's scale: with t = score + log2(v_scale), P = 2^(t - max t) is at most 1 for every row,
+//     whatever the sizes of the blocks' values. It is rounded to f16 (2^-11; from 2^10 down to 2^-24, so
+//     nothing within 2^-34 of the row's largest is lost); the denominator is summed in f32 before that.
+//   * f32 queries: Q and P as the sum of two f16 values each, two products in place of one.
+#include <cuda_fp16.h>
 #include <math.h>
 
+#include <mutex>
+
 #include "kv_cache.cuh"
+#include "umma_ptx.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kThreads = 128;
+constexpr int kTileTokens = 64;
+constexpr int kWarps = 8;                 // workers of a CTA, one CTA per SM
+constexpr float kHeadroom = 10.f;         // P = 2^(t - max + 10) ...
+constexpr float kStale = 5.f;             // ... and the maximum may be 5 behind: at most 2^15 in f16
+constexpr float kSmallestScale = 7.888609052210118e-31f;
+constexpr int kErrCachedWait = 1024;
 
 struct CachedParams {
   Cache cache;
@@ -21,61 +51,544 @@ struct CachedParams {
   int64_t q_batch, q_token, q_head;
   const int32_t* lengths;
   int32_t batch, tokens, heads, group;
+  int32_t rows, row_tiles;  // query rows of a (sequence, key/value head): tokens * group, row = token * group + head within the group
+  int32_t workers;
   float scale_log2;
+  float* partial;  // [workers][2][rows of a tile x (2 + dim)]
   int32_t* status;
 };
 
-// One CTA per (sequence, token, query head): a thread scores one position of a tile of 128, then sums
-// one channel over the tile.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) cached_simple_kernel(const CachedParams p) {
-  __shared__ float query[D], prob[kThreads], value_scale[kThreads], part[4];
-  __shared__ int64_t where[kThreads];
+__device__ const float g_not_a_number = __builtin_nanf("");
+
+__device__ __forceinline__ int64_t capacity_of(const CachedParams& p) {
+  return static_cast<int64_t>(p.table.width) << p.cache.token_bits;
+}
+// Tiles of one (sequence, head, row tile). A sequence that its table cannot hold has none: it is answered with NaN.
+__device__ __forceinline__ int64_t tiles_of(const CachedParams& p, int32_t b) {
+  const int64_t length = p.lengths[b];
+  return length <= 0 || length > capacity_of(p) ? 0 : (length + kTileTokens - 1) / kTileTokens;
+}
+__device__ __forceinline__ int64_t total_tiles(const CachedParams& p) {
+  int64_t sum = 0;
+  for (int32_t b = threadIdx.x & 31; b < p.batch; b += 32) sum += tiles_of(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * p.cache.heads * p.row_tiles;
+}
+__device__ __forceinline__ int64_t tiles_per_worker(const CachedParams& p, int64_t total) {
+  return (total + p.workers - 1) / p.workers;
+}
+template <int ROWS, int D>
+__device__ __forceinline__ float* partial_of(const CachedParams& p, int64_t worker, int slot) {
+  return p.partial + (worker * 2 + slot) * (ROWS * (2 + D));
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Of f32 values the part that f16 leaves over.
+__device__ __forceinline__ uint32_t half2_rest(float lo, float hi, uint32_t rounded) {
+  const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
+  return half2_bits(lo - r.x, hi - r.y);
+}
+// Four codes to f16: bytes 0, 1 and bytes 2, 3.
+__device__ __forceinline__ void codes_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  const uint32_t biased = codes ^ 0x80808080u;
+  lo = __byte_perm(biased, 0x64646464u, 0x4140);
+  hi = __byte_perm(biased, 0x64646464u, 0x4342);
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+  const __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), bias), b = __hsub2(*reinterpret_cast<__half2*>(&hi), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void word_load(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// Arrives (without raising the expected count) when this thread's word_loads so far have landed.
+__device__ __forceinline__ void word_loads_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Where a worker stands in the line of tiles.
+struct Cursor {
+  int32_t b, h, rt;
+  int64_t tile, tiles;
+};
+__device__ __forceinline__ void advance(const CachedParams& p, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.rt < p.row_tiles) return;
+  c.rt = 0;
+  if (++c.h < p.cache.heads) return;
+  c.h = 0;
+  do {
+    ++c.b;
+    c.tiles = c.b < p.batch ? tiles_of(p, c.b) : 1;  // behind the last one: never used
+  } while (c.tiles == 0);
+}
+
+template <int D>
+struct Ring {
+  static constexpr int kSlots = D == 64 ? 6 : 3;
+  // 64 tokens of a head, plus the gap between pages that keeps V's columns on different banks
+  static constexpr uint32_t kSlotBytes = kTileTokens * D + 128;
+  static constexpr uint32_t kScaleBytes = 4 * 8 * 4;  // of four tiles: four pages' K and V scales
+  static constexpr uint32_t kWarpBytes = kSlots * kSlotBytes + kScaleBytes;
+  static constexpr size_t kBytes = 128 + kWarps * (kWarpBytes + kSlots * 8) + 16;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedParams p) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr int kRows = 8 * NT, kSteps = D / 16, kSlots = Ring<D>::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = lane & 3, octet = lane >> 2;  // fragment coordinates: column pair, row
+  uint8_t* base = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+  uint8_t* ring = base + warp * Ring<D>::kWarpBytes;
+  float* scales = reinterpret_cast<float*>(ring + kSlots * Ring<D>::kSlotBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kWarps * Ring<D>::kWarpBytes) + warp * kSlots;
+  volatile int* abort_flag = reinterpret_cast<int*>(base + kWarps * (Ring<D>::kWarpBytes + kSlots * 8));
+  const uint32_t ring_addr = smem_u32(ring), scales_addr = smem_u32(scales), bars_addr = smem_u32(bars);
+  if (lane == 0) {
+    for (int s = 0; s < kSlots; ++s) mbar_init(bars_addr + 8 * s, 33);
+    fence_barrier_init();
+  }
+  if (threadIdx.x == 0) *abort_flag = 0;
+  __syncthreads();
+
   const Cache& c = p.cache;
-  const int head = blockIdx.x, token = blockIdx.y, b = blockIdx.z, kv_head = head / p.group;
-  T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.tokens + token) * p.heads + head) * D;
-  const int64_t limit = static_cast<int64_t>(p.lengths[b]) - p.tokens + token + 1;
-  if (threadIdx.x < D)
-    query[threadIdx.x] =
-        Elem<T>::load(static_cast<const T*>(p.q) + b * p.q_batch + token * p.q_token + head * p.q_head + threadIdx.x);
-  float top = -INFINITY, total = 0.f, acc = 0.f;
-  for (int64_t tile = 0; tile < limit; tile += kThreads) {
-    __syncthreads();
-    const int64_t position = tile + threadIdx.x;
-    float s = -INFINITY;
-    if (position < limit) {
-      const int64_t block = block_of(c, p.table, b, position >> c.token_bits, p.status);
-      where[threadIdx.x] = block;
-      value_scale[threadIdx.x] = __uint_as_float(0x7fc00000u);
-      s = value_scale[threadIdx.x];
-      if (block >= 0) {
-        const int8_t* k = c.k_codes + (block * c.heads + kv_head) * c.tokens * D + (position & (c.tokens - 1)) * D;
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = fmaf(query[d], k[d], s);
-        s *= c.k_scales[block * c.heads + kv_head] * p.scale_log2;
-        value_scale[threadIdx.x] = c.v_scales[block * c.heads + kv_head];
+  const int64_t total = total_tiles(p), each = tiles_per_worker(p, total);
+  // neighbouring workers on different SMs: little work spreads over all of them
+  const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
+  const int64_t begin = worker * each, end = min(begin + each, total);
+  if (worker >= p.workers || begin >= end) return;
+
+  Cursor at;
+  {
+    const Piece piece = find_piece(p.batch, begin, [&](int32_t b) { return tiles_of(p, b) * c.heads * p.row_tiles; });
+    at.b = piece.sequence;
+    at.tiles = tiles_of(p, at.b);
+    const int64_t pair = piece.index / at.tiles;
+    at.tile = piece.index - pair * at.tiles;
+    at.h = static_cast<int32_t>(pair / p.row_tiles);
+    at.rt = static_cast<int32_t>(pair - static_cast<int64_t>(at.h) * p.row_tiles);
+  }
+
+  // -------------------------------------------------------------------- copies
+  // Item 2u is the K tile of the worker's u-th unit, item 2u + 1 its V tile; item i goes to slot i % kSlots.
+  // Items are issued in order; lane i copies the tile's i-th page.
+  const int pages_full = kTileTokens >> c.token_bits;
+  const uint32_t page_bytes = static_cast<uint32_t>(D) << c.token_bits;
+  const uint32_t v_page_step = page_bytes + (c.token_bits == 4 ? 32u : 64u);
+  const int64_t units = end - begin, items = 2 * units;
+  Cursor ahead = at;
+  int64_t next_item = 0;
+  uint32_t next_slot = 0;
+  int32_t next_block = -1;
+  bool next_held = false;  // whether a position of this lane's page exists
+  auto look_up = [&]() {   // the block of this lane's page of the next unit
+    const int64_t page = ahead.tile * pages_full + lane;
+    const int64_t held = (static_cast<int64_t>(p.lengths[ahead.b]) + c.tokens - 1) >> c.token_bits;
+    next_held = lane < pages_full && page < held;
+    next_block = next_held ? p.table.blocks[ahead.b * p.table.stride + page] : -1;
+  };
+  auto issue = [&]() {
+    const uint32_t bar = bars_addr + 8 * next_slot;
+    const bool is_v = next_item & 1;
+    const bool there = next_block >= 0 && next_block < c.blocks;
+    const unsigned copies = __ballot_sync(0xffffffffu, there);
+    if (lane == 0) mbar_expect_tx(bar, __popc(copies) * page_bytes);
+    __syncwarp();
+    const int64_t pair = static_cast<int64_t>(next_block) * c.heads + ahead.h;
+    if (there) {
+      const uint32_t dst = ring_addr + next_slot * Ring<D>::kSlotBytes + lane * (is_v ? v_page_step : page_bytes);
+      bulk_load(dst, (is_v ? c.v_codes : c.k_codes) + pair * page_bytes, page_bytes, bar);
+    }
+    if (!is_v && next_held) {
+      const uint32_t dst = scales_addr + (static_cast<uint32_t>(next_item >> 1) & 3u) * 32 + lane * 4;
+      word_load(dst, there ? c.k_scales + pair : &g_not_a_number);
+      word_load(dst + 16, there ? c.v_scales + pair : &g_not_a_number);
+      if (!there && p.status) atomicOr(p.status, kErrBlocks);
+    }
+    word_loads_arrive(bar);
+    if (++next_slot == kSlots) next_slot = 0;
+    if ((++next_item & 1) == 0 && next_item < items) {
+      advance(p, ahead);
+      look_up();
+    }
+  };
+  look_up();
+  for (int i = 0; i < kSlots && next_item < items; ++i) issue();
+
+  // -------------------------------------------------------------------- the work
+  uint32_t slot = 0, parity = 0;
+  auto arrived = [&]() {
+    bool ok = mbar_wait(bars_addr + 8 * slot, parity, abort_flag, p.status, kErrCachedWait);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+  auto release = [&]() {
+    __syncwarp();
+    if (++slot == kSlots) {
+      slot = 0;
+      parity ^= 1u;
+    }
+    if (next_item < items) issue();
+  };
+
+  uint32_t q_hi[kSteps][NT][2], q_lo[kSplit ? kSteps : 1][kSplit ? NT : 1][2];
+  float o[kSteps][NT][4], row_scale[NT][2], top[NT][2], sum[NT][2];
+  int64_t limit[NT][2];  // positions that the row sees
+  int64_t segment = begin - at.tile;
+  bool fresh = true;
+
+  for (int64_t unit = begin; unit < end; ++unit) {
+    if (fresh) {
+      // Queries of this (sequence, head): row `octet` of each row tile, the 16 consecutive dims per 64 that
+      // belong to this quad; scaled by a power of two that brings the row's largest to [1, 2).
+      fresh = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int row = at.rt * kRows + n * 8 + octet;
+        float x[D / 4];
+        uint32_t largest = 0;
+        const bool real = row < p.rows;
+        const int token = row / p.group, head = at.h * p.group + row % p.group;
+        const T* src = static_cast<const T*>(p.q) + at.b * p.q_batch + token * p.q_token + head * p.q_head;
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) {
+          x[i] = real ? Elem<T>::load(src + (i / 16) * 64 + quad * 16 + i % 16) : 0.f;
+          largest = max(largest, __float_as_uint(x[i]) & 0x7fffffffu);
+        }
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        const uint32_t power = min(max(largest & 0x7f800000u, 27u << 23), 253u << 23);
+        const float down = __uint_as_float((254u << 23) - power);
+        float up = __uint_as_float(power) * p.scale_log2;
+        if (largest >= 0x7f800000u) up = __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float lo = x[4 * s + 2 * e] * down, hi = x[4 * s + 2 * e + 1] * down;
+            q_hi[s][n][e] = half2_bits(lo, hi);
+            if (kSplit) q_lo[s][n][e] = half2_rest(lo, hi, q_hi[s][n][e]);
+          }
+        const int64_t length = p.lengths[at.b];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          row_scale[n][e] = __shfl_sync(0xffffffffu, up, (2 * quad + e) * 4);
+          limit[n][e] = length - p.tokens + 1 + (at.rt * kRows + n * 8 + 2 * quad + e) / p.group;
+          top[n][e] = -INFINITY;
+          sum[n][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[s][n][i] = 0.f;
+    }
+
+    // S^T = K Q^T. Row r of 16-row tile m is token 16 (r % 8 / 2) + 4 m + 2 (r / 8) + r % 2: what a thread
+    // gets of a row is then, transposed, the four consecutive tokens that its bytes of V hold.
+    if (!arrived()) break;
+    const float* tile_scales = scales + (static_cast<uint32_t>(unit - begin) & 3u) * 8;
+    const int page = (octet >> 1) >> (c.token_bits - 4);
+    const float k_scale = tile_scales[page];
+    const float v_raw = tile_scales[4 + page], v_scale = v_raw < kSmallestScale ? kSmallestScale : v_raw;
+    float s[4][NT][4];
+    {
+      const uint8_t* tile = ring + slot * Ring<D>::kSlotBytes + (16 * (octet >> 1) + (octet & 1)) * D + quad * 16;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
+#pragma unroll
+        for (int half = 0; half < D / 64; ++half) {
+          const uint4 first = *reinterpret_cast<const uint4*>(tile + 4 * m * D + half * 64);
+          const uint4 second = *reinterpret_cast<const uint4*>(tile + (4 * m + 2) * D + half * 64);
+          const uint32_t w0[4] = {first.x, first.y, first.z, first.w}, w1[4] = {second.x, second.y, second.z, second.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a[4];
+            codes_to_half(w0[i], a[0], a[2]);
+            codes_to_half(w1[i], a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_f16(s[m][n], a, q_hi[half * 4 + i][n][0], q_hi[half * 4 + i][n][1]);
+              if (kSplit) mma_f16(s[m][n], a, q_lo[half * 4 + i][n][0], q_lo[half * 4 + i][n][1]);
+            }
+          }
+        }
       }
     }
-    const float warp_best = warp_fmax(s);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = warp_best;
-    __syncthreads();
-    const float best = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), top);
-    const float base = best == -INFINITY ? 0.f : best;
-    const float keep = fast_exp2(top - base);
-    top = best;
-    prob[threadIdx.x] = position < limit ? fast_exp2(s - base) : 0.f;
-    __syncthreads();
-    total *= keep;
-    acc *= keep;
-    const int here = static_cast<int>(limit - tile < kThreads ? limit - tile : kThreads);
-    for (int j = 0; j < here; ++j) {
-      total += prob[j];
-      if (threadIdx.x >= D) continue;
-      const int64_t at = (where[j] * c.heads + kv_head) * c.tokens * D + threadIdx.x * c.tokens + ((tile + j) & (c.tokens - 1));
-      acc = fmaf(prob[j], (where[j] < 0 ? 1.f : static_cast<float>(c.v_codes[at])) * value_scale[j], acc);
+    release();
+
+    // Softmax: this thread has 8 tokens of two rows for each row tile.
+    const float v_log = log2f(v_scale);
+    const int64_t first_token = at.tile * kTileTokens + 16 * (octet >> 1) + (octet & 1);
+    const bool cut = at.tile * kTileTokens + kTileTokens > p.lengths[at.b] - p.tokens + 1;
+    uint32_t p_hi[4][NT][2], p_lo[kSplit ? 4 : 1][kSplit ? NT : 1][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float factor = row_scale[n][e] * k_scale;
+        float best = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& x = s[m][n][2 * h + e];
+            x *= factor;
+            if (cut && first_token + 4 * m + 2 * h >= limit[n][e]) x = -INFINITY;
+            best = fmaxf(best, x);
+          }
+        best = best == -INFINITY ? best : best + v_log;  // (a masked position's scale may be anything)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+        if (__any_sync(0xffffffffu, best > top[n][e] + kStale)) {
+          const float higher = fmaxf(best, top[n][e]);
+          const float keep = higher == -INFINITY ? 1.f : fast_exp2(top[n][e] - higher);
+          top[n][e] = higher;
+          sum[n][e] *= keep;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            o[i][n][e] *= keep;
+            o[i][n][2 + e] *= keep;
+          }
+        }
+        const float shift = (top[n][e] == -INFINITY ? 0.f : top[n][e]) - kHeadroom;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& x = s[m][n][2 * h + e];
+            const bool masked = cut && x == -INFINITY;
+            x = fast_exp2(x - shift);
+            sum[n][e] += x;
+            x = masked ? 0.f : x * v_scale;
+          }
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t pair = half2_bits(s[m][n][2 * h], s[m][n][2 * h + 1]);
+          p_hi[m][n][h] = transpose_8x8(pair);
+          if (kSplit) p_lo[m][n][h] = transpose_8x8(half2_rest(s[m][n][2 * h], s[m][n][2 * h + 1], pair));
+        }
+    }
+
+    // O^T += V^T P^T: a thread's 16 bytes of a channel are 16 tokens, four for each of the four products.
+    if (!arrived()) break;
+    {
+      const int in_page = quad & ((1 << (c.token_bits - 4)) - 1);
+      const uint8_t* tile = ring + slot * Ring<D>::kSlotBytes + (quad >> (c.token_bits - 4)) * v_page_step + in_page * 16;
+#pragma unroll
+      for (int d = 0; d < kSteps; ++d) {
+        const uint4 first = *reinterpret_cast<const uint4*>(tile + ((16 * d + octet) << c.token_bits));
+        const uint4 second = *reinterpret_cast<const uint4*>(tile + ((16 * d + octet + 8) << c.token_bits));
+        const uint32_t w0[4] = {first.x, first.y, first.z, first.w}, w1[4] = {second.x, second.y, second.z, second.w};
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          uint32_t a[4];
+          codes_to_half(w0[m], a[0], a[2]);
+          codes_to_half(w1[m], a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_f16(o[d][n], a, p_hi[m][n][0], p_hi[m][n][1]);
+            if (kSplit) mma_f16(o[d][n], a, p_lo[m][n][0], p_lo[m][n][1]);
+          }
+        }
+      }
+    }
+    release();
+
+    if (at.tile + 1 == at.tiles || unit + 1 == end) {
+      const bool whole = segment >= begin && at.tile + 1 == at.tiles;
+      float* left = partial_of<kRows, D>(p, worker, segment >= begin ? 1 : 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float l = sum[n][e];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+          const int in_tile = n * 8 + 2 * quad + e, row = at.rt * kRows + in_tile;
+          if (row >= p.rows) continue;
+          if (whole) {
+            const float inv = limit[n][e] <= 0 ? 0.f : 1.f / l;
+            const int token = row / p.group, head = at.h * p.group + row % p.group;
+            T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(at.b) * p.tokens + token) * p.heads + head) * D;
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d) {
+              Elem<T>::store(dst + 16 * d + octet, o[d][n][e] * inv);
+              Elem<T>::store(dst + 16 * d + octet + 8, o[d][n][2 + e] * inv);
+            }
+          } else {
+            if (octet == 0) {
+              left[in_tile] = top[n][e];
+              left[kRows + in_tile] = l;
+            }
+            float* dst = left + 2 * kRows + in_tile * D;
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d) {
+              dst[16 * d + octet] = o[d][n][e];
+              dst[16 * d + octet + 8] = o[d][n][2 + e];
+            }
+          }
+        }
+      fresh = true;
+      segment = unit + 1;
+    }
+    if (unit + 1 < end) advance(p, at);
+  }
+  if (*abort_flag) {
+    // A wait ran out: copies of this warp may still be in flight; give them (bounded) time to land.
+    const unsigned long long start = global_ns();
+    while (global_ns() - start < 2000000ull) {
     }
   }
-  if (threadIdx.x < D) Elem<T>::store(out + threadIdx.x, limit <= 0 ? 0.f : acc / total);
+}
+
+// Joins what several workers left of one row: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w. One CTA per
+// (sequence, head, row tile) and row; its warps take the workers in turn, and their sums are added in the order of the warps.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) cached_join_kernel(const CachedParams p) {
+  constexpr int kRows = 8 * NT, kPer = D / 32;
+  __shared__ float best_of[8], sum_of[8], acc_of[8][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t pairs = static_cast<int64_t>(p.cache.heads) * p.row_tiles;
+  const int32_t b = static_cast<int32_t>(blockIdx.x / pairs);
+  const int64_t pair = blockIdx.x - b * pairs;
+  const int32_t h = static_cast<int32_t>(pair / p.row_tiles), rt = static_cast<int32_t>(pair - h * static_cast<int64_t>(p.row_tiles));
+  const int in_tile = blockIdx.y, row = rt * kRows + in_tile;
+  if (row >= p.rows) return;
+  const int token = row / p.group;
+  const int64_t length = p.lengths[b], limit = length - p.tokens + 1 + token;
+  T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.tokens + token) * p.heads + h * p.group + row % p.group) * D;
+  const int64_t tiles = tiles_of(p, b);
+  if (tiles == 0) {
+    const bool beyond = length > 0;
+    if (beyond && threadIdx.x == 0 && p.status) atomicOr(p.status, kErrBlocks);
+    if (threadIdx.x < D) Elem<T>::store(dst + threadIdx.x, beyond ? __uint_as_float(0x7fc00000u) : 0.f);
+    return;
+  }
+  int64_t before = 0, all = 0;
+  for (int32_t i = lane; i < p.batch; i += 32) {
+    const int64_t t = tiles_of(p, i);
+    all += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const int64_t each = tiles_per_worker(p, all * pairs), start = before * pairs + pair * tiles;
+  const int64_t first = start / each, last = (start + tiles - 1) / each;
+  if (first == last) return;  // finished by its worker
+  auto left_by = [&](int64_t w) { return partial_of<kRows, D>(p, w, start >= w * each ? 1 : 0); };
+
+  float best = -INFINITY;
+  for (int64_t w = first + threadIdx.x; w <= last; w += 256) best = fmaxf(best, left_by(w)[in_tile]);
+  best = warp_fmax(best);
+  if (lane == 0) best_of[warp] = best;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) best = fmaxf(best, best_of[i]);
+  if (best == -INFINITY) best = 0.f;
+  float sum = 0.f, acc[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int64_t w = first + warp; w <= last; w += 8) {
+    const float* left = left_by(w);
+    const float weight = fast_exp2(left[in_tile] - best);
+    sum = fmaf(left[kRows + in_tile], weight, sum);
+    const float* x = left + 2 * kRows + in_tile * D + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(x[i], weight, acc[i]);
+  }
+  if (lane == 0) sum_of[warp] = sum;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc_of[warp][lane * kPer + i] = acc[i];
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float total = 0.f, value = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    total += sum_of[i];
+    value += acc_of[i][threadIdx.x];
+  }
+  Elem<T>::store(dst + threadIdx.x, limit <= 0 ? 0.f : value / total);
+}
+
+// Query rows of a tile: 8, or 16 where a (sequence, head) has more than 8 (32 would not leave room in
+// the registers for the accumulators beside the queries).
+int row_tile(int64_t rows) { return rows <= 8 ? 8 : 16; }
+
+struct CachedPlan {
+  int64_t rows, row_tiles, pairs, workers;
+  int tile, grid;
+};
+CachedPlan plan_cached(const b200_kv_cache* c, int64_t batch, int64_t tokens, int64_t heads, int64_t table_width, int sms) {
+  CachedPlan plan{};
+  plan.rows = tokens * (heads / c->heads);
+  plan.tile = row_tile(plan.rows);
+  plan.row_tiles = ceil_div(plan.rows, plan.tile);
+  plan.pairs = batch * c->heads * plan.row_tiles;
+  // no more workers than the longest possible sequences have tiles
+  const int64_t most = plan.pairs * (ceil_div(table_width * c->block_tokens, kTileTokens) + 1);
+  plan.grid = static_cast<int>(most < sms ? most : sms);
+  plan.workers = most < static_cast<int64_t>(plan.grid) * kWarps ? most : static_cast<int64_t>(plan.grid) * kWarps;
+  return plan;
+}
+
+std::once_flag g_cached_attr_once[64];
+
+template <typename T, int D, int NT>
+int launch_cached(const CachedParams& p, const CachedPlan& plan, cudaStream_t s) {
+  cached_kernel<T, D, NT><<<plan.grid, 32 * kWarps, Ring<D>::kBytes, s>>>(p);
+  const int code = check_launch();
+  if (code) return finish(code);
+  cached_join_kernel<T, D, NT><<<dim3(static_cast<unsigned>(plan.pairs), 8 * NT), 256, 0, s>>>(p);
+  return launched();
+}
+template <typename T>
+void cached_attributes() {
+  cudaFuncSetAttribute(cached_kernel<T, 64, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<64>::kBytes));
+  cudaFuncSetAttribute(cached_kernel<T, 64, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<64>::kBytes));
+  cudaFuncSetAttribute(cached_kernel<T, 128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<128>::kBytes));
+  cudaFuncSetAttribute(cached_kernel<T, 128, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<128>::kBytes));
+}
+template <typename T>
+int launch_cached_any(const CachedParams& p, const CachedPlan& plan, int dim, cudaStream_t s) {
+  if (dim == 64) return plan.tile == 8 ? launch_cached<T, 64, 1>(p, plan, s) : launch_cached<T, 64, 2>(p, plan, s);
+  return plan.tile == 8 ? launch_cached<T, 128, 1>(p, plan, s) : launch_cached<T, 128, 2>(p, plan, s);
 }
 
 }  // namespace
@@ -85,7 +598,12 @@ using namespace b200;
 
 extern "C" size_t b200_attention_cached_workspace_bytes(const b200_kv_cache* cache, int64_t batch, int64_t tokens,
                                                         int64_t heads, int64_t table_width) {
-  return 0;
+  if (!cache || !valid_cache(cache) || batch < 1 || tokens < 1 || heads < 1 || heads % cache->heads || table_width < 0 ||
+      table_width > INT32_MAX)
+    return 0;
+  const int sms = device_info().sm_count;
+  const CachedPlan plan = plan_cached(cache, batch, tokens, heads, table_width, sms);
+  return static_cast<size_t>(plan.workers) * 2 * plan.tile * (2 + cache->dim) * sizeof(float);
 }
 
 extern "C" int b200_attention_cached(const b200_kv_cache* cache, int32_t dtype, const void* q, int64_t q_batch,
@@ -96,14 +614,23 @@ extern "C" int b200_attention_cached(const b200_kv_cache* cache, int32_t dtype, 
   if (!enabled()) return refuse(B200_E_DISABLED);
   if (!cache) return refuse(B200_E_NULL);
   if (!valid_dtype(dtype)) return refuse(B200_E_DTYPE);
-  if (!valid_cache(cache) || batch < 0 || tokens < 0 || heads < 1 || heads % cache->heads || batch > 65535 || tokens > 65535)
+  if (!valid_cache(cache) || batch < 0 || tokens < 0 || heads < 1 || heads % cache->heads || batch > INT32_MAX / 8 ||
+      tokens > INT32_MAX / 8 || heads > INT32_MAX / 8)
     return refuse(B200_E_SHAPE);
   if (!(fabsf(scale) <= 3.0e38f)) return refuse(B200_E_ARG);
   if (batch == 0 || tokens == 0) return finish(0);
-  if (!cache_pointers(cache) || !q || !out || !lengths) return refuse(B200_E_NULL);
+  if (!cache_pointers(cache) || !q || !out || !lengths || (table_width > 0 && !block_table)) return refuse(B200_E_NULL);
   if (table_width < 0 || table_width > INT32_MAX || (batch > 1 && table_stride < table_width)) return refuse(B200_E_STRIDE);
-  if (!cache_aligned(cache)) return refuse(B200_E_ALIGN);
-  if (device_info().sm_count == 0) return refuse(B200_E_DEVICE);
+  if (!cache_aligned(cache) || !aligned(q, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)) || !aligned(block_table, 4) ||
+      !aligned(lengths, 4))
+    return refuse(B200_E_ALIGN);
+  const DeviceInfo& dev = device_info();
+  if (dev.sm_count == 0) return refuse(B200_E_DEVICE);
+  const CachedPlan plan = plan_cached(cache, batch, tokens, heads, table_width, dev.sm_count);
+  if (plan.rows > INT32_MAX / 2 || plan.pairs > INT32_MAX) return refuse(B200_E_SHAPE);
+  if (!workspace || workspace_bytes < b200_attention_cached_workspace_bytes(cache, batch, tokens, heads, table_width) ||
+      !aligned(workspace, 16))
+    return refuse(B200_E_WORKSPACE);
   CachedParams p{};
   p.cache = device_cache(cache);
   p.table = Table{block_table, table_stride, static_cast<int32_t>(table_width)};
@@ -117,17 +644,17 @@ extern "C" int b200_attention_cached(const b200_kv_cache* cache, int32_t dtype, 
   p.tokens = static_cast<int32_t>(tokens);
   p.heads = static_cast<int32_t>(heads);
   p.group = static_cast<int32_t>(heads / cache->heads);
+  p.rows = static_cast<int32_t>(plan.rows);
+  p.row_tiles = static_cast<int32_t>(plan.row_tiles);
+  p.workers = static_cast<int32_t>(plan.workers);
   p.scale_log2 = scale * kLog2e;
+  p.partial = static_cast<float*>(workspace);
   p.status = kernel_status_word();
+  std::call_once(g_cached_attr_once[dev.device], [] {
+    cached_attributes<float>();
+    cached_attributes<__nv_bfloat16>();
+  });
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(tokens), static_cast<unsigned>(batch));
-  if (dtype == B200_F32 && cache->dim == 64)
-    cached_simple_kernel<float, 64><<<grid, kThreads, 0, s>>>(p);
-  else if (dtype == B200_F32)
-    cached_simple_kernel<float, 128><<<grid, kThreads, 0, s>>>(p);
-  else if (cache->dim == 64)
-    cached_simple_kernel<__nv_bfloat16, 64><<<grid, kThreads, 0, s>>>(p);
-  else
-    cached_simple_kernel<__nv_bfloat16, 128><<<grid, kThreads, 0, s>>>(p);
-  return launched();
+  return dtype == B200_F32 ? launch_cached_any<float>(p, plan, cache->dim, s)
+                           : launch_cached_any<__nv_bfloat16>(p, plan, cache->dim, s);
 }

@@ -206,7 +206,9 @@ def _explain_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], blo
                     scale: float | None = None) -> CallExplanation:
     _, heads, dim = _describe(cache, "attention_cached")
     _check_cached(q, heads, dim, _table("attention_cached", block_table)[0])
-    return CallExplanation(True, "cached_simple_kernel")
+    tokens = 1 if q.dim() == 3 else q.shape[1]
+    rows = tokens * (q.shape[-2] // heads)
+    return CallExplanation(True, f"cached_kernel (mma f16, {8 if rows <= 8 else 16} query rows a tile, {rows} rows a head) + cached_join_kernel")
 
 
 attention_cached.explain = _explain_cached  # type: ignore[attr-defined]
