@@ -5,11 +5,13 @@
 // [offsets[b], offsets[b + 1]). Causal: the queries are the last positions of the keys, so
 // row i sees keys j <= i + keys - queries. A row that sees no key is zeros, and so are the
 // rows behind the last sequence. No reference counterpart.
+#include <cuda.h>
 #include <math.h>
 
 #include <mutex>
 
 #include "sequences.cuh"
+#include "umma_ptx.cuh"
 
 namespace b200 {
 namespace {
@@ -215,6 +217,499 @@ void launch_simt_any(const PackedParams& p, cudaStream_t s) {
     launch_simt<T, 256>(p, s);
 }
 
+// ------------------------------------------------------------------------- bf16, head size 64 or 128
+// The tensor-core form. A CTA takes two tiles of 128 query rows over the same keys: the same rows of two
+// query heads that share a key/value head, or, where the heads do not come in such pairs, 256
+// rows of one head. Each block of 128 keys is loaded once for both.
+//   warps 0-3, 4-7  softmax of tile 0, 1: thread = query row = TMEM lane. It takes its 128 scores from tensor memory,
+//                   keeps the running maximum and sum, writes P = 2^(score - maximum) as bf16 pairs over the scores (tcgen05.st)
+//                   in two halves, each signalled when it is there, and rescales its row of the output
+//                   accumulator only when the maximum grew by more than 2^8 (a stale maximum
+//                   scales numerator and denominator alike).
+//   warp 8          TMA: lane 0 Q and the K blocks, lane 1 the V blocks
+//   warp 9          MMA issue: for each block, tile 0 then tile 1: O += P V (A from tensor memory), then the next S = Q K^T
+// The tiles run half a period apart: while the tensor core works for one, the other's exponentials are
+// computed. A tile's period is softmax + P V + Q K^T, since P lies where its scores were (tensor memory is full:
+// 2 x 128 columns of scores, 2 x 128 of output), so the softmax's own length counts in full. It is
+// kept short by registers for the whole row (setmaxnreg) and by taking a part of the exponentials off the
+// special-function unit (16 a cycle and SM: 1024 cycles a block, as long as the two products).
+// Masks cost only the blocks that they cut. A value that a row does not see still meets P = 0 in the product, and
+// 0 * infinity would be NaN: a row whose result is not finite looks whether such a value lay in the blocks that its mask cuts, and
+// is computed again without the tensor core if so.
+constexpr int kQRows = 128, kKeys = 128;
+constexpr int kUmmaThreads = 384, kUmmaProducerWarp = 8, kUmmaMmaWarp = 9;
+constexpr uint32_t kUmmaScoreCols = 128, kUmmaOutCol = 256;
+constexpr float kRescale = 8.0f;
+constexpr int kErrPackedWait = 2048;
+
+template <int D>
+struct UmmaTile {
+  static constexpr int kChunks = D / 64;  // 64-element column chunks
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr uint32_t kBytes = kChunks * 16384;  // 128 rows x D bf16
+  static constexpr uint32_t kVHalf = kChunks * 8192;   // 64 keys x D bf16
+};
+
+struct __align__(8) UmmaBarriers {
+  uint64_t q_full[2];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t s_full[2], p_full[2][2], o_done[2];  // by tile (and half of the keys)
+  uint32_t tmem_base;
+  int abort_flag;
+};
+template <int D>
+constexpr size_t umma_smem_bytes() {
+  return 1024 + (2 + 2 * UmmaTile<D>::kStages) * UmmaTile<D>::kBytes + sizeof(UmmaBarriers);
+}
+
+struct UmmaParams {
+  PackedParams p;
+  int32_t pairs;       // pairs of tiles in a row of pieces: heads / 2, or heads
+  int32_t head_pairs;  // 1: the two tiles are two heads; 0: two runs of rows
+  uint32_t idesc_qk, idesc_pv;
+};
+
+// One row again, by one thread: what the tensor core cannot do without touching unseen values.
+template <int D>
+__device__ __forceinline__ void packed_row_again(const PackedParams& p, const __nv_bfloat16* q, const __nv_bfloat16* k,
+                                              const __nv_bfloat16* v, int64_t sees, int64_t read, __nv_bfloat16* dst) {
+  bool touched = false;
+  for (int64_t j = sees; j < read && !touched; ++j)
+    for (int d = 0; d < D; d += 8) {
+      const uint4 w = ld_plain16(v + j * p.v_row + d);
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        touched |= (words[i] & 0x7f80u) == 0x7f80u || (words[i] & 0x7f800000u) == 0x7f800000u;
+    }
+  if (!touched) return;  // the row itself is not finite
+  float acc[D], top = -INFINITY, total = 0.f;
+  for (int d = 0; d < D; ++d) acc[d] = 0.f;
+  for (int64_t j = 0; j < sees; ++j) {
+    float s = 0.f;
+    for (int d = 0; d < D; d += 8) {
+      float a[8], b[8];
+      unpack16(ld_plain16(q + d), a);
+      unpack16(ld_plain16(k + j * p.k_row + d), b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+    }
+    s *= p.scale_log2;
+    const float best = fmaxf(top, s), base = best == -INFINITY ? 0.f : best;
+    const float keep = fast_exp2(top - base), weight = fast_exp2(s - base);
+    top = best;
+    total = fmaf(total, keep, weight);
+    for (int d = 0; d < D; d += 8) {
+      float b[8];
+      unpack16(ld_plain16(v + j * p.v_row + d), b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[d + i] = fmaf(weight, b[i], acc[d + i] * keep);
+    }
+  }
+  const float inv = 1.f / total;
+  for (int d = 0; d < D; ++d) dst[d] = __float2bfloat16_rn(acc[d] * inv);
+}
+
+// 2^x for two values on the FMA pipe, |relative error| < 8.6e-5 (P is rounded to 2^-9): x = n + r with n the whole number below
+// (adding 1.5 * 2^23 rounded down), a cubic for 2^r over [0, 1) that is 1 at 0 and was fitted for the least
+// largest relative error, and n added to the exponent bits. At and below -127 the result is exactly 0, so that
+// a masked or vanishing score does not even carry a huge value along.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& lo, float& hi) {
+  float a, b;
+  unpack_f32x2(x, a, b);
+  x = pack_f32x2(fmaxf(a, -127.f), fmaxf(b, -127.f));
+  const uint64_t magic = pack_f32x2(12582912.f, 12582912.f), back = pack_f32x2(-12582912.f, -12582912.f);
+  uint64_t shifted;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(shifted) : "l"(x), "l"(magic));
+  const uint64_t r = fma_f32x2(add_f32x2(shifted, back), pack_f32x2(-1.f, -1.f), x);
+  uint64_t y = fma_f32x2(r, pack_f32x2(0.077067241f, 0.077067241f), pack_f32x2(0.22764498f, 0.22764498f));
+  y = fma_f32x2(y, r, pack_f32x2(0.69511664f, 0.69511664f));
+  y = fma_f32x2(y, r, pack_f32x2(1.f, 1.f));
+  float n0, n1;
+  unpack_f32x2(shifted, n0, n1);
+  unpack_f32x2(y, lo, hi);
+  lo = __int_as_float(__float_as_int(lo) + (__float_as_int(n0) << 23));
+  hi = __int_as_float(__float_as_int(hi) + (__float_as_int(n1) << 23));
+}
+
+__device__ __forceinline__ float nan_fmax(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kUmmaThreads, 1)
+    packed_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ UmmaParams u) {
+  constexpr int kChunks = UmmaTile<D>::kChunks, kStages = UmmaTile<D>::kStages;
+  constexpr uint32_t kTileBytes = UmmaTile<D>::kBytes, kVHalfBytes = UmmaTile<D>::kVHalf;
+  extern __shared__ uint8_t smem_raw[];
+  const PackedParams& p = u.p;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_smem = smem_base;
+  const uint32_t k_smem = q_smem + 2 * kTileBytes;
+  const uint32_t v_smem = k_smem + kStages * kTileBytes;
+  const uint32_t end_smem = v_smem + kStages * kTileBytes;
+  UmmaBarriers* bars = reinterpret_cast<UmmaBarriers*>(smem_raw + (end_smem - smem_u32(smem_raw)));
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Which piece: the last rows of a sequence, which see the most keys, come first.
+  const int rows_each = u.head_pairs ? kQRows : 2 * kQRows;
+  const int64_t pieces = gridDim.x / u.pairs;
+  const int64_t place = blockIdx.x / u.pairs;
+  const int pair = static_cast<int>(blockIdx.x - place * u.pairs);
+  const Piece piece = find_piece(p.batch, pieces - 1 - place, [&](int32_t b) {
+    return (rows_of(p.offsets, b, p.rows_q, p.status).count + rows_each - 1) / rows_each;
+  });
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
+  if (piece.sequence < 0) {
+    const Rows rest = rows_behind(p.offsets, p.batch, p.rows_q);
+    const int64_t first = piece.index * rows_each;
+    const int heads_here = u.head_pairs ? 2 : 1, head0 = u.head_pairs ? 2 * pair : pair;
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(rows_each) * heads_here * (D / 8); i += kUmmaThreads) {
+      const int64_t r = first + i / (heads_here * (D / 8));
+      const int part = static_cast<int>(i % (heads_here * (D / 8)));
+      if (r < rest.count)
+        *reinterpret_cast<uint4*>(out + ((rest.begin + r) * p.heads + head0) * D + part * 8) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const Rows mine = rows_of(p.offsets, piece.sequence, p.rows_q, nullptr);
+  const Rows theirs = rows_of(p.k_offsets, piece.sequence, p.rows_k, p.status);
+  const int64_t shift = p.causal ? theirs.count - mine.count + 1 : 0;  // row i sees the keys below i + shift
+  int64_t row0[2], keys[2];
+  int rows[2], head[2], blocks[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    head[t] = u.head_pairs ? 2 * pair + t : pair;
+    row0[t] = piece.index * rows_each + (u.head_pairs ? 0 : t * kQRows);
+    const int64_t left = mine.count - row0[t];
+    rows[t] = static_cast<int>(left < 0 ? 0 : (left < kQRows ? left : kQRows));
+    keys[t] = theirs.count;
+    if (p.causal && row0[t] + rows[t] - 1 + shift < keys[t]) keys[t] = row0[t] + rows[t] - 1 + shift;
+    if (rows[t] == 0 || keys[t] < 0) keys[t] = 0;
+    blocks[t] = static_cast<int>((keys[t] + kKeys - 1) / kKeys);
+  }
+  const int most = max(blocks[0], blocks[1]);
+  const int kv_head = head[0] / p.group;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&bars->q_full[t]), 1);
+      mbar_init(smem_u32(&bars->s_full[t]), 1);
+      mbar_init(smem_u32(&bars->p_full[t][0]), 4);
+      mbar_init(smem_u32(&bars->p_full[t][1]), 4);
+      mbar_init(smem_u32(&bars->o_done[t]), 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(smem_u32(&bars->k_full[s]), 1);
+      mbar_init(smem_u32(&bars->k_empty[s]), 1);
+      mbar_init(smem_u32(&bars->v_full[s]), 1);
+      mbar_init(smem_u32(&bars->v_empty[s]), 1);
+    }
+    bars->abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == kUmmaMmaWarp) {
+    tmem_alloc<1>(smem_u32(&bars->tmem_base), 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp >= 8) {
+    // 384 threads x 168 registers at launch = 128 x (2 x 208 + 88)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int key_begin = static_cast<int>(theirs.begin);
+    if (warp == kUmmaProducerWarp && lane < 2) {
+      // ---------------------------------------------------------------- TMA producers
+      if (lane == 0) {
+        for (int t = 0; t < 2; ++t) {
+          if (!blocks[t]) continue;
+          const uint32_t qf = smem_u32(&bars->q_full[t]);
+          mbar_expect_tx(qf, kTileBytes);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d(q_smem + t * kTileBytes + c * 16384, &map_q, qf, 64 * c, static_cast<int>(mine.begin + row0[t]), head[t]);
+        }
+      }
+      uint32_t stage = 0, parity = 1;  // a fresh barrier's preceding phase counts as complete
+      for (int j = 0; j < most; ++j) {
+        const uint32_t empty = smem_u32(lane == 0 ? &bars->k_empty[stage] : &bars->v_empty[stage]);
+        const uint32_t full = smem_u32(lane == 0 ? &bars->k_full[stage] : &bars->v_full[stage]);
+        if (!mbar_wait(empty, parity, abort_flag, p.status, kErrPackedWait)) break;
+        mbar_expect_tx(full, kTileBytes);
+        if (lane == 0) {
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d(k_smem + stage * kTileBytes + c * 16384, &map_k, full, 64 * c, key_begin + j * kKeys, kv_head);
+        } else {
+          for (int h = 0; h < 2; ++h)
+            for (int c = 0; c < kChunks; ++c)
+              tma_load_3d(v_smem + stage * kTileBytes + h * kVHalfBytes + c * 8192, &map_v, full, 64 * c,
+                          key_begin + j * kKeys + 64 * h, kv_head);
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+      if (*abort_flag) {
+        // Loads that were issued may still be in flight: give them (bounded) time to land.
+        const unsigned long long start = global_ns();
+        while (global_ns() - start < 2000000ull) {
+        }
+      }
+    } else if (warp == kUmmaMmaWarp && lane == 0) {
+      // ---------------------------------------------------------------- MMA issuer
+      const uint32_t hi = desc_hi(1024);
+      bool ok = true;
+      auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T, both K-major
+        const uint64_t q_desc = make_desc(q_smem + t * kTileBytes, 1u, hi);
+        const uint64_t k_desc = make_desc(k_smem + (j % kStages) * kTileBytes, 1u, hi);
+        const uint32_t d_tmem = tmem_base + t * kUmmaScoreCols;
+#pragma unroll
+        for (int i = 0; i < kChunks * 4; ++i) {
+          const uint64_t step = static_cast<uint64_t>(((i >> 2) * 16384 + (i & 3) * 32) >> 4);
+          umma_bf16<1>(d_tmem, q_desc + step, k_desc + step, u.idesc_qk, i ? 1u : 0u);
+        }
+        umma_commit<1>(smem_u32(&bars->s_full[t]));
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && mbar_wait(smem_u32(bar), parity, abort_flag, p.status, kErrPackedWait);
+        tc_fence_after();
+        return ok;
+      };
+      if (most > 0 && wait(&bars->k_full[0], 0)) {
+        for (int t = 0; t < 2 && ok; ++t)
+          if (blocks[t] && wait(&bars->q_full[t], 0)) scores(t, 0);
+        umma_commit<1>(smem_u32(&bars->k_empty[0]));
+      }
+      for (int j = 0; j < most && ok; ++j) {
+        const uint32_t st = j % kStages, next = (j + 1) % kStages;
+        const uint64_t v_lo = make_desc(v_smem + st * kTileBytes, 8192u >> 4, hi);
+        const uint64_t v_hi = make_desc(v_smem + st * kTileBytes + kVHalfBytes, 8192u >> 4, hi);
+        if (!wait(&bars->v_full[st], (j / kStages) & 1)) break;
+        if (j + 1 < most && !wait(&bars->k_full[next], ((j + 1) / kStages) & 1)) break;
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= blocks[t]) continue;
+          const uint32_t d_tmem = tmem_base + kUmmaOutCol + t * D, p_tmem = tmem_base + t * kUmmaScoreCols;
+          if (!wait(&bars->p_full[t][0], j & 1)) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            umma_bf16_ts(d_tmem, p_tmem + i * 8, v_lo + static_cast<uint64_t>((i * 2048) >> 4), u.idesc_pv, (j | i) ? 1u : 0u);
+          if (!wait(&bars->p_full[t][1], j & 1)) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            umma_bf16_ts(d_tmem, p_tmem + 32 + i * 8, v_hi + static_cast<uint64_t>((i * 2048) >> 4), u.idesc_pv, 1u);
+          umma_commit<1>(smem_u32(&bars->o_done[t]));
+          // The next scores go where P lies; the tensor core runs what one thread issues in order.
+          if (j + 1 < blocks[t]) scores(t, j + 1);
+        }
+        umma_commit<1>(smem_u32(&bars->v_empty[st]));
+        if (j + 1 < most) umma_commit<1>(smem_u32(&bars->k_empty[next]));
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax and output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t score_addr = tmem_base + lane_addr + t * kUmmaScoreCols;
+    const uint32_t out_addr = tmem_base + lane_addr + kUmmaOutCol + t * D;
+    const int64_t my_row0 = t ? row0[1] : row0[0], my_keys = t ? keys[1] : keys[0];
+    const int my_rows = t ? rows[1] : rows[0], my_blocks = t ? blocks[1] : blocks[0], my_head = t ? head[1] : head[0];
+    // keys that this row sees, and those that every row of the tile sees
+    int64_t sees = theirs.count, all_see = theirs.count;
+    if (p.causal) {
+      sees = min(max(my_row0 + row + shift, int64_t{0}), theirs.count);
+      all_see = min(max(my_row0 + shift, int64_t{0}), theirs.count);
+    }
+    const uint32_t s_full = smem_u32(&bars->s_full[t]), o_done = smem_u32(&bars->o_done[t]);
+    const uint32_t p_half0 = smem_u32(&bars->p_full[t][0]), p_half1 = smem_u32(&bars->p_full[t][1]);
+    float top = -1.0e30f, total = 0.f;
+    bool ok = true;
+    for (int j = 0; j < my_blocks; ++j) {
+      ok = mbar_wait(s_full, j & 1, abort_flag, p.status, kErrPackedWait);
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      if (!ok) break;
+      tc_fence_after();
+      float s[kKeys];
+      {
+        uint32_t(&raw)[kKeys] = reinterpret_cast<uint32_t(&)[kKeys]>(s);
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32(score_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(raw[c * 32]));
+        tmem_ld_wait();
+      }
+      if (static_cast<int64_t>(j + 1) * kKeys > all_see) {
+        const int64_t here = sees - static_cast<int64_t>(j) * kKeys;
+        const int valid = static_cast<int>(here < kKeys ? here : kKeys);
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i)
+          if (i >= valid) s[i] = -INFINITY;
+      }
+      float part[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[i] = s[i];
+#pragma unroll
+      for (int i = 8; i < kKeys; ++i) part[i & 7] = nan_fmax(part[i & 7], s[i]);
+#pragma unroll
+      for (int i = 4; i > 0; i >>= 1)
+#pragma unroll
+        for (int x = 0; x < i; ++x) part[x] = nan_fmax(part[x], part[x + i]);
+      const float best = nan_fmax(top, part[0] * p.scale_log2);
+      if (__any_sync(0xffffffffu, !(best - top <= kRescale))) {
+        // Some row of this warp outgrew its maximum, or is not finite (it stays NaN from here on).
+        const float higher = best < INFINITY ? best : __uint_as_float(0x7fc00000u);
+        const float alpha = fast_exp2(top - higher);
+        total *= alpha;
+        top = higher;
+        if (j > 0) {
+          ok = mbar_wait(o_done, (j - 1) & 1, abort_flag, p.status, kErrPackedWait);
+          ok = __all_sync(0xffffffffu, ok) != 0;
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t raw[16];
+            tmem_ld_32x16(out_addr + c * 16, raw);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * alpha);
+            tmem_st_32x16(out_addr + c * 16, raw);
+          }
+          tmem_st_wait();
+        }
+      }
+      const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), neg_top2 = pack_f32x2(-top, -top);
+      uint64_t sums[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          const uint64_t x = fma_f32x2(pack_f32x2(s[h * 64 + i], s[h * 64 + i + 1]), scale2, neg_top2);
+          float lo, hi;
+          if ((i & 6) == 6) {  // one pair of four on the FMA pipe
+            exp2_pair(x, lo, hi);
+          } else {
+            unpack_f32x2(x, lo, hi);
+            lo = fast_exp2(lo);
+            hi = fast_exp2(hi);
+          }
+          sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(lo, hi));
+          packed[i >> 1] = pack_bf16x2(lo, hi);
+        }
+        tmem_st_32x32(score_addr + h * 32, packed);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(h ? p_half1 : p_half0);
+      }
+      float lo, hi;
+      unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), lo, hi);
+      total += lo + hi;
+    }
+    if (ok && my_blocks > 0) {
+      ok = mbar_wait(o_done, (my_blocks - 1) & 1, abort_flag, p.status, kErrPackedWait);
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      tc_fence_after();
+    }
+    if (ok) {
+      const float inv = sees > 0 ? 1.f / total : 0.f;
+      __nv_bfloat16* dst = out + ((mine.begin + my_row0 + row) * p.heads + my_head) * D;
+      uint32_t largest = 0;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
+        if (my_blocks > 0) {
+          tmem_ld_32x32(out_addr + c * 32, x);
+          tmem_ld_wait();
+        }
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          o[i] = sees > 0 ? __uint_as_float(x[i]) * inv : 0.f;
+          largest = max(largest, __float_as_uint(o[i]) & 0x7fffffffu);
+        }
+        if (row < my_rows) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v8[8] = {o[8 * i],     o[8 * i + 1], o[8 * i + 2], o[8 * i + 3],
+                                 o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]};
+            *reinterpret_cast<uint4*>(dst + c * 32 + 8 * i) = pack16(v8);
+          }
+        }
+      }
+      if (largest >= 0x7f800000u && row < my_rows) {
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + (mine.begin + my_row0 + row) * p.q_row + my_head * p.q_head;
+        const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k) + theirs.begin * p.k_row + kv_head * p.k_head;
+        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v) + theirs.begin * p.v_row + kv_head * p.v_head;
+        const int64_t read = min(static_cast<int64_t>(my_blocks) * kKeys, p.rows_k - theirs.begin);
+        packed_row_again<D>(p, q, k, v, sees, read, dst);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kUmmaMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, 512);
+  }
+}
+
+uint32_t umma_idesc(int n, bool b_kmajor) {
+  uint32_t d = 0;
+  d |= 1u << 4;   // D format f32
+  d |= 1u << 7;   // A format bf16
+  d |= 1u << 10;  // B format bf16
+  d |= (b_kmajor ? 0u : 1u) << 16;
+  d |= static_cast<uint32_t>(n >> 3) << 17;
+  d |= static_cast<uint32_t>(kQRows >> 4) << 24;
+  return d;
+}
+
+std::once_flag g_umma_attr_once[64];
+
+bool tma_strides(const void* base, int64_t row, int64_t head) {
+  return aligned(base, 16) && row > 0 && head > 0 && row % 8 == 0 && head % 8 == 0 && row < (int64_t{1} << 38) &&
+         head < (int64_t{1} << 38);
+}
+// The tensor-core form takes bf16 heads of 64 and 128 with a positive scale (its maximum is that of the raw scores) and
+// strides that a TMA descriptor can hold.
+bool umma_takes(const b200_packed_attention_desc& d) {
+  return d.dtype == B200_BF16 && (d.dim == 64 || d.dim == 128) && d.scale > 0.f && d.rows_k > 0 &&
+         tma_strides(d.q, d.q_row, d.q_head) && tma_strides(d.k, d.k_row, d.k_head) && tma_strides(d.v, d.v_row, d.v_head) &&
+         aligned(d.out, 16);
+}
+
+template <int D>
+int launch_umma(const PackedParams& p, const b200_packed_attention_desc& d, cudaStream_t s) {
+  UmmaParams u{};
+  u.p = p;
+  // Pairs of heads share every key block and mask, and leave tiles of 128 rows; an odd group pairs rows instead.
+  u.head_pairs = p.group % 2 == 0;
+  u.pairs = u.head_pairs ? p.heads / 2 : p.heads;
+  const int64_t pieces = p.rows_q / (u.head_pairs ? kQRows : 2 * kQRows) + p.batch + 1;
+  if (pieces * u.pairs > INT32_MAX) return refuse(B200_E_SHAPE);
+  u.idesc_qk = umma_idesc(kKeys, true);
+  u.idesc_pv = umma_idesc(D, false);
+  CUtensorMap map_q, map_k, map_v;
+  if (!encode_map(&map_q, d.q, D, d.rows_q, d.heads, d.q_row, d.q_head, 64, kQRows) ||
+      !encode_map(&map_k, d.k, D, d.rows_k, d.kv_heads, d.k_row, d.k_head, 64, kKeys) ||
+      !encode_map(&map_v, d.v, D, d.rows_k, d.kv_heads, d.v_row, d.v_head, 64, 64))
+    return refuse(B200_E_DEVICE);
+  packed_umma_kernel<D><<<static_cast<unsigned>(pieces * u.pairs), kUmmaThreads, umma_smem_bytes<D>(), s>>>(map_q, map_k, map_v, u);
+  return launched();
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -267,6 +762,13 @@ extern "C" int b200_attention_packed(const b200_packed_attention_desc* desc, voi
     simt_attributes<float>();
     simt_attributes<__nv_bfloat16>();
   });
+  std::call_once(g_umma_attr_once[dev.device], [] {
+    cudaFuncSetAttribute(packed_umma_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(umma_smem_bytes<64>()));
+    cudaFuncSetAttribute(packed_umma_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(umma_smem_bytes<128>()));
+  });
+  if (umma_takes(d)) return d.dim == 64 ? launch_umma<64>(p, d, s) : launch_umma<128>(p, d, s);
   if (d.dtype == B200_F32)
     launch_simt_any<float>(p, s);
   else

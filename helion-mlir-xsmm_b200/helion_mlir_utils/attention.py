@@ -115,6 +115,19 @@ def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: T
         raise ValueError(f"attention_packed() needs k_offsets where k has other rows than q: {tuple(q.shape)}, {tuple(k.shape)}")
 
 
+def _tensor_core(q: Tensor, scale: float | None) -> bool:
+    """Whether the tcgen05 kernel takes these operands (else f32 tiles on the CUDA cores)."""
+    return q.dtype == torch.bfloat16 and q.shape[2] in _FUSED_DIMS and (scale is None or 0.0 < scale < math.inf)
+
+
+def _for_tma(t: Tensor) -> Tensor:
+    """``t`` if a TMA descriptor can hold its strides, else a contiguous copy."""
+    row, head, dim = t.stride()
+    if dim == 1 and row > 0 and head > 0 and row % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _packed_desc(q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, offsets: Tensor, k_offsets: Tensor, scale: float,
                  causal: bool) -> native.PackedAttentionDesc:
     rows, heads, dim = q.shape
@@ -142,7 +155,10 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
     _check_packed(q, k, v, offsets, k_offsets)
     device = native.require_cuda(q, k, v, offsets, k_offsets)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
+    if _tensor_core(q, scale):
+        q, k, v = _for_tma(q), _for_tma(k), _for_tma(v)
+    else:
+        q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
     with native.on_device(device):
         out = output_pool.empty(tuple(q.shape), dtype=q.dtype, device=device)
         desc = _packed_desc(q, k, v, out, offsets, k_offsets, scale, bool(causal))
@@ -154,6 +170,8 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
 def _explain_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor | None = None,
                     scale: float | None = None, causal: bool = True) -> CallExplanation:
     _check_packed(q, k, v, offsets, offsets if k_offsets is None else k_offsets)
+    if _tensor_core(q, scale):
+        return CallExplanation(True, "packed_umma_kernel (tcgen05, two tiles of 128 queries x 128 keys per step, scores in TMEM)")
     return CallExplanation(True, "packed_simt_kernel (f32 tiles of 64 x 64)")
 
 
