@@ -231,8 +231,15 @@ void launch_simt_any(const PackedParams& p, cudaStream_t s) {
 // The tiles run half a period apart: while the tensor core works for one, the other's exponentials are
 // computed. A tile's period is softmax + P V + Q K^T, since P lies where its scores were (tensor memory is full:
 // 2 x 128 columns of scores, 2 x 128 of output), so the softmax's own length counts in full. It is
-// kept short by registers for the whole row (setmaxnreg) and by taking a part of the exponentials off the
-// special-function unit (16 a cycle and SM: 1024 cycles a block, as long as the two products).
+// kept short by registers for the whole row (setmaxnreg), three-input maxima and by taking a part of the exponentials off the
+// special-function unit (16 a cycle and SM: 1024 cycles a block, as long as the two products). What bounds it now is
+// that softmax: of the 3210 cycles of a period a group works 1950 (maximum 250, exponentials 1420, the rest loads, stores
+// and signals: one warp to a scheduler hides little of its own latencies) and waits 1250 for the products, which the other
+// group's work covers only in part. One sequence of 8192, 32/8 heads of 128: 1174 TFLOP/s in short runs, 1045 sustained
+// under the power cap (0.71 and 0.75 of measured cuBLAS). Measured and not kept there: P in columns of its own with blocks
+// of 80 keys, which ends the waiting but costs more softmax and MMA time a key (519 against 482 us); 16 softmax warps, two to a
+// row (496); taking turns at the exponentials (506); the maximum taken alongside stale exponentials (519); a cubic
+// for 0, 1/4 or 3/8 of the exponentials in place of 1/8 (491, 482, 530 against 468).
 // Masks cost only the blocks that they cut. A value that a row does not see still meets P = 0 in the product, and
 // 0 * infinity would be NaN: a row whose result is not finite looks whether such a value lay in the blocks that its mask cuts, and
 // is computed again without the tensor core if so.
@@ -332,9 +339,10 @@ __device__ __forceinline__ void exp2_pair(uint64_t x, float& lo, float& hi) {
   hi = __int_as_float(__float_as_int(hi) + (__float_as_int(n1) << 23));
 }
 
-__device__ __forceinline__ float nan_fmax(float a, float b) {
+// The larger of three, NaN if one is.
+__device__ __forceinline__ float nan_fmax(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -556,14 +564,17 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
       }
       float part[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) part[i] = s[i];
+      for (int i = 0; i < 8; ++i) part[i] = nan_fmax(s[i], s[i + 8], s[i + 16]);
 #pragma unroll
-      for (int i = 8; i < kKeys; ++i) part[i & 7] = nan_fmax(part[i & 7], s[i]);
+      for (int i = 24; i < kKeys - 8; i += 16)
 #pragma unroll
-      for (int i = 4; i > 0; i >>= 1)
+        for (int x = 0; x < 8; ++x) part[x] = nan_fmax(part[x], s[i + x], s[i + 8 + x]);
 #pragma unroll
-        for (int x = 0; x < i; ++x) part[x] = nan_fmax(part[x], part[x + i]);
-      const float best = nan_fmax(top, part[0] * p.scale_log2);
+      for (int x = 0; x < 4; ++x) part[x] = nan_fmax(part[x], s[kKeys - 8 + x], s[kKeys - 4 + x]);
+      part[0] = nan_fmax(part[0], part[1], part[2]);
+      part[3] = nan_fmax(part[3], part[4], part[5]);
+      part[6] = nan_fmax(part[6], part[7], part[0]);
+      const float raw = nan_fmax(part[3], part[6], part[6]) * p.scale_log2, best = nan_fmax(top, raw, raw);
       if (__any_sync(0xffffffffu, !(best - top <= kRescale))) {
         // Some row of this warp outgrew its maximum, or is not finite (it stays NaN from here on).
         const float higher = best < INFINITY ? best : __uint_as_float(0x7fc00000u);
@@ -596,7 +607,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         for (int i = 0; i < 64; i += 2) {
           const uint64_t x = fma_f32x2(pack_f32x2(s[h * 64 + i], s[h * 64 + i + 1]), scale2, neg_top2);
           float lo, hi;
-          if ((i & 6) == 6) {  // one pair of four on the FMA pipe
+          if ((i & 14) == 14) {  // one pair of eight on the FMA pipe
             exp2_pair(x, lo, hi);
           } else {
             unpack_f32x2(x, lo, hi);
