@@ -555,14 +555,14 @@ struct CachedPlan {
   int64_t rows, row_tiles, pairs, workers;
   int tile, grid;
 };
-CachedPlan plan_cached(const b200_kv_cache* c, int64_t batch, int64_t tokens, int64_t heads, int64_t table_width, int sms) {
+CachedPlan plan_cached(const b200_cached_attention_desc& d, int sms) {
   CachedPlan plan{};
-  plan.rows = tokens * (heads / c->heads);
+  plan.rows = d.tokens * (d.heads / d.cache.heads);
   plan.tile = row_tile(plan.rows);
   plan.row_tiles = ceil_div(plan.rows, plan.tile);
-  plan.pairs = batch * c->heads * plan.row_tiles;
+  plan.pairs = d.batch * d.cache.heads * plan.row_tiles;
   // no more workers than the longest possible sequences have tiles
-  const int64_t most = plan.pairs * (ceil_div(table_width * c->block_tokens, kTileTokens) + 1);
+  const int64_t most = plan.pairs * (ceil_div(d.table_width * d.cache.block_tokens, kTileTokens) + 1);
   plan.grid = static_cast<int>(most < sms ? most : sms);
   plan.workers = most < static_cast<int64_t>(plan.grid) * kWarps ? most : static_cast<int64_t>(plan.grid) * kWarps;
   return plan;
@@ -596,65 +596,66 @@ int launch_cached_any(const CachedParams& p, const CachedPlan& plan, int dim, cu
 
 using namespace b200;
 
-extern "C" size_t b200_attention_cached_workspace_bytes(const b200_kv_cache* cache, int64_t batch, int64_t tokens,
-                                                        int64_t heads, int64_t table_width) {
-  if (!cache || !valid_cache(cache) || batch < 1 || tokens < 1 || heads < 1 || heads % cache->heads || table_width < 0 ||
-      table_width > INT32_MAX)
-    return 0;
-  const int sms = device_info().sm_count;
-  const CachedPlan plan = plan_cached(cache, batch, tokens, heads, table_width, sms);
-  return static_cast<size_t>(plan.workers) * 2 * plan.tile * (2 + cache->dim) * sizeof(float);
+static size_t workspace_for(const CachedPlan& plan, int dim) {
+  return static_cast<size_t>(plan.workers) * 2 * plan.tile * (2 + dim) * sizeof(float);
 }
 
-extern "C" int b200_attention_cached(const b200_kv_cache* cache, int32_t dtype, const void* q, int64_t q_batch,
-                                     int64_t q_token, int64_t q_head, void* out, const int32_t* block_table,
-                                     int64_t table_stride, int64_t table_width, const int32_t* lengths, int64_t batch,
-                                     int64_t tokens, int64_t heads, float scale, void* workspace, size_t workspace_bytes,
-                                     void* stream) {
+extern "C" int64_t b200_attention_cached_workspace_bytes(const b200_cached_attention_desc* desc) {
+  if (!desc) return 0;
+  const b200_cached_attention_desc& d = *desc;
+  if (!valid_cache(&d.cache) || d.batch < 1 || d.tokens < 1 || d.heads < 1 || d.heads % d.cache.heads || d.table_width < 0 ||
+      d.table_width > INT32_MAX)
+    return 0;
+  return static_cast<int64_t>(workspace_for(plan_cached(d, device_info().sm_count), d.cache.dim));
+}
+
+extern "C" int b200_attention_cached(const b200_cached_attention_desc* desc, void* stream) {
   if (!enabled()) return refuse(B200_E_DISABLED);
-  if (!cache) return refuse(B200_E_NULL);
-  if (!valid_dtype(dtype)) return refuse(B200_E_DTYPE);
-  if (!valid_cache(cache) || batch < 0 || tokens < 0 || heads < 1 || heads % cache->heads || batch > INT32_MAX / 8 ||
-      tokens > INT32_MAX / 8 || heads > INT32_MAX / 8)
+  if (!desc) return refuse(B200_E_NULL);
+  const b200_cached_attention_desc& d = *desc;
+  if (!valid_dtype(d.dtype)) return refuse(B200_E_DTYPE);
+  if (!valid_cache(&d.cache) || d.batch < 0 || d.tokens < 0 || d.heads < 1 || d.heads % d.cache.heads ||
+      d.batch > INT32_MAX / 8 || d.tokens > INT32_MAX / 8 || d.heads > INT32_MAX / 8)
     return refuse(B200_E_SHAPE);
-  if (!(fabsf(scale) <= 3.0e38f)) return refuse(B200_E_ARG);
-  if (batch == 0 || tokens == 0) return finish(0);
-  if (!cache_pointers(cache) || !q || !out || !lengths || (table_width > 0 && !block_table)) return refuse(B200_E_NULL);
-  if (table_width < 0 || table_width > INT32_MAX || (batch > 1 && table_stride < table_width)) return refuse(B200_E_STRIDE);
-  if (!cache_aligned(cache) || !aligned(q, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)) || !aligned(block_table, 4) ||
-      !aligned(lengths, 4))
+  if (!(fabsf(d.scale) <= 3.0e38f)) return refuse(B200_E_ARG);
+  if (d.batch == 0 || d.tokens == 0) return finish(0);
+  if (!cache_pointers(&d.cache) || !d.q || !d.out || !d.lengths || (d.table_width > 0 && !d.block_table))
+    return refuse(B200_E_NULL);
+  if (d.table_width < 0 || d.table_width > INT32_MAX || (d.batch > 1 && d.table_stride < d.table_width))
+    return refuse(B200_E_STRIDE);
+  if (!cache_aligned(&d.cache) || !aligned(d.q, dtype_size(d.dtype)) || !aligned(d.out, dtype_size(d.dtype)) ||
+      !aligned(d.block_table, 4) || !aligned(d.lengths, 4))
     return refuse(B200_E_ALIGN);
   const DeviceInfo& dev = device_info();
   if (dev.sm_count == 0) return refuse(B200_E_DEVICE);
-  const CachedPlan plan = plan_cached(cache, batch, tokens, heads, table_width, dev.sm_count);
+  const CachedPlan plan = plan_cached(d, dev.sm_count);
   if (plan.rows > INT32_MAX / 2 || plan.pairs > INT32_MAX) return refuse(B200_E_SHAPE);
-  if (!workspace || workspace_bytes < b200_attention_cached_workspace_bytes(cache, batch, tokens, heads, table_width) ||
-      !aligned(workspace, 16))
+  if (!d.workspace || d.workspace_bytes < static_cast<int64_t>(workspace_for(plan, d.cache.dim)) || !aligned(d.workspace, 16))
     return refuse(B200_E_WORKSPACE);
   CachedParams p{};
-  p.cache = device_cache(cache);
-  p.table = Table{block_table, table_stride, static_cast<int32_t>(table_width)};
-  p.q = q;
-  p.out = out;
-  p.q_batch = q_batch;
-  p.q_token = q_token;
-  p.q_head = q_head;
-  p.lengths = lengths;
-  p.batch = static_cast<int32_t>(batch);
-  p.tokens = static_cast<int32_t>(tokens);
-  p.heads = static_cast<int32_t>(heads);
-  p.group = static_cast<int32_t>(heads / cache->heads);
+  p.cache = device_cache(&d.cache);
+  p.table = Table{d.block_table, d.table_stride, static_cast<int32_t>(d.table_width)};
+  p.q = d.q;
+  p.out = d.out;
+  p.q_batch = d.q_batch;
+  p.q_token = d.q_token;
+  p.q_head = d.q_head;
+  p.lengths = d.lengths;
+  p.batch = static_cast<int32_t>(d.batch);
+  p.tokens = static_cast<int32_t>(d.tokens);
+  p.heads = static_cast<int32_t>(d.heads);
+  p.group = static_cast<int32_t>(d.heads / d.cache.heads);
   p.rows = static_cast<int32_t>(plan.rows);
   p.row_tiles = static_cast<int32_t>(plan.row_tiles);
   p.workers = static_cast<int32_t>(plan.workers);
-  p.scale_log2 = scale * kLog2e;
-  p.partial = static_cast<float*>(workspace);
+  p.scale_log2 = d.scale * kLog2e;
+  p.partial = static_cast<float*>(d.workspace);
   p.status = kernel_status_word();
   std::call_once(g_cached_attr_once[dev.device], [] {
     cached_attributes<float>();
     cached_attributes<__nv_bfloat16>();
   });
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == B200_F32 ? launch_cached_any<float>(p, plan, cache->dim, s)
-                           : launch_cached_any<__nv_bfloat16>(p, plan, cache->dim, s);
+  return d.dtype == B200_F32 ? launch_cached_any<float>(p, plan, d.cache.dim, s)
+                             : launch_cached_any<__nv_bfloat16>(p, plan, d.cache.dim, s);
 }

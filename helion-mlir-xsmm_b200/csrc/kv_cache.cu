@@ -271,82 +271,82 @@ bool table_ok(const int32_t* table, int64_t batch, int64_t stride, int64_t width
 
 using namespace b200;
 
-extern "C" int b200_kv_append(const b200_kv_cache* cache, int32_t dtype, const void* k, const void* v, int64_t k_row,
-                              int64_t k_head, int64_t v_row, int64_t v_head, const int32_t* block_table,
-                              int64_t table_stride, int64_t table_width, const int32_t* lengths, const int32_t* offsets,
-                              int64_t batch, int64_t rows, void* stream) {
+extern "C" int b200_kv_append(const b200_kv_append_desc* desc, void* stream) {
   if (!enabled()) return refuse(B200_E_DISABLED);
-  if (!cache) return refuse(B200_E_NULL);
-  if (!valid_dtype(dtype)) return refuse(B200_E_DTYPE);
-  if (!valid_cache(cache) || batch < 0 || rows < 0 || rows > INT32_MAX || batch > INT32_MAX / 8) return refuse(B200_E_SHAPE);
-  if (!offsets && batch > 0 && rows % batch) return refuse(B200_E_SHAPE);
-  if (batch == 0 || rows == 0) return finish(0);
-  if (!cache_pointers(cache) || !k || !v || !lengths) return refuse(B200_E_NULL);
-  if (!table_ok(block_table, batch, table_stride, table_width)) return refuse(B200_E_STRIDE);
-  const int64_t vec = dtype == B200_F32 ? 4 : 8;
-  if (k_row % vec || k_head % vec || v_row % vec || v_head % vec) return refuse(B200_E_STRIDE);
-  if (!cache_aligned(cache) || !aligned(k, 16) || !aligned(v, 16) || !aligned(block_table, 4) || !aligned(lengths, 4) ||
-      !aligned(offsets, 4))
+  if (!desc) return refuse(B200_E_NULL);
+  const b200_kv_append_desc& d = *desc;
+  if (!valid_dtype(d.dtype)) return refuse(B200_E_DTYPE);
+  if (!valid_cache(&d.cache) || d.batch < 0 || d.rows < 0 || d.rows > INT32_MAX || d.batch > INT32_MAX / 8)
+    return refuse(B200_E_SHAPE);
+  if (!d.offsets && d.batch > 0 && d.rows % d.batch) return refuse(B200_E_SHAPE);
+  if (d.batch == 0 || d.rows == 0) return finish(0);
+  if (!cache_pointers(&d.cache) || !d.k || !d.v || !d.lengths) return refuse(B200_E_NULL);
+  if (!table_ok(d.block_table, d.batch, d.table_stride, d.table_width)) return refuse(B200_E_STRIDE);
+  const int64_t vec = d.dtype == B200_F32 ? 4 : 8;
+  if (d.k_row % vec || d.k_head % vec || d.v_row % vec || d.v_head % vec) return refuse(B200_E_STRIDE);
+  if (!cache_aligned(&d.cache) || !aligned(d.k, 16) || !aligned(d.v, 16) || !aligned(d.block_table, 4) ||
+      !aligned(d.lengths, 4) || !aligned(d.offsets, 4))
     return refuse(B200_E_ALIGN);
   if (device_info().sm_count == 0) return refuse(B200_E_DEVICE);
   AppendParams p{};
-  p.cache = device_cache(cache);
-  p.table = Table{block_table, table_stride, static_cast<int32_t>(table_width)};
-  p.k = k;
-  p.v = v;
-  p.k_row = k_row;
-  p.k_head = k_head;
-  p.v_row = v_row;
-  p.v_head = v_head;
-  p.lengths = lengths;
-  p.offsets = offsets;
-  p.rows = rows;
-  p.batch = static_cast<int32_t>(batch);
-  p.each = offsets ? 0 : static_cast<int32_t>(rows / batch);
+  p.cache = device_cache(&d.cache);
+  p.table = Table{d.block_table, d.table_stride, static_cast<int32_t>(d.table_width)};
+  p.k = d.k;
+  p.v = d.v;
+  p.k_row = d.k_row;
+  p.k_head = d.k_head;
+  p.v_row = d.v_row;
+  p.v_head = d.v_head;
+  p.lengths = d.lengths;
+  p.offsets = d.offsets;
+  p.rows = d.rows;
+  p.batch = static_cast<int32_t>(d.batch);
+  p.each = d.offsets ? 0 : static_cast<int32_t>(d.rows / d.batch);
   p.status = kernel_status_word();
   // n new tokens touch at most (n - 2) / tokens + 2 blocks; one token each, one block each
-  const int64_t pieces = !offsets && rows == batch ? batch : rows / cache->block_tokens + 2 * batch;
-  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(cache->heads), 2);
-  const unsigned threads = static_cast<unsigned>(cache->block_tokens / 4 * (cache->dim / 8));
+  const int64_t pieces = !d.offsets && d.rows == d.batch ? d.batch : d.rows / d.cache.block_tokens + 2 * d.batch;
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(d.cache.heads), 2);
+  const unsigned threads = static_cast<unsigned>(d.cache.block_tokens / 4 * (d.cache.dim / 8));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == B200_F32)
+  if (d.dtype == B200_F32)
     kv_append_kernel<float><<<grid, threads, 0, s>>>(p);
   else
     kv_append_kernel<__nv_bfloat16><<<grid, threads, 0, s>>>(p);
   return launched();
 }
 
-extern "C" int b200_kv_read(const b200_kv_cache* cache, int32_t dtype, void* k_out, void* v_out, const int32_t* block_table,
-                            int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths,
-                            const int32_t* offsets, int64_t batch, int64_t rows, void* stream) {
+extern "C" int b200_kv_read(const b200_kv_read_desc* desc, void* stream) {
   if (!enabled()) return refuse(B200_E_DISABLED);
-  if (!cache) return refuse(B200_E_NULL);
-  if (!valid_dtype(dtype)) return refuse(B200_E_DTYPE);
-  if (!valid_cache(cache) || batch < 0 || rows < 0 || rows > INT32_MAX || batch > INT32_MAX / 8) return refuse(B200_E_SHAPE);
-  if (rows == 0) return finish(0);
-  if (!cache_pointers(cache) || !k_out || !v_out || !offsets || (batch > 0 && (!starts || !lengths))) return refuse(B200_E_NULL);
-  if (!table_ok(block_table, batch, table_stride, table_width)) return refuse(B200_E_STRIDE);
-  if (!cache_aligned(cache) || !aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(block_table, 4) ||
-      !aligned(starts, 4) || !aligned(lengths, 4) || !aligned(offsets, 4))
+  if (!desc) return refuse(B200_E_NULL);
+  const b200_kv_read_desc& d = *desc;
+  if (!valid_dtype(d.dtype)) return refuse(B200_E_DTYPE);
+  if (!valid_cache(&d.cache) || d.batch < 0 || d.rows < 0 || d.rows > INT32_MAX || d.batch > INT32_MAX / 8)
+    return refuse(B200_E_SHAPE);
+  if (d.rows == 0) return finish(0);
+  if (!cache_pointers(&d.cache) || !d.k_out || !d.v_out || !d.offsets || (d.batch > 0 && (!d.starts || !d.lengths)))
+    return refuse(B200_E_NULL);
+  if (!table_ok(d.block_table, d.batch, d.table_stride, d.table_width)) return refuse(B200_E_STRIDE);
+  if (!cache_aligned(&d.cache) || !aligned(d.k_out, 16) || !aligned(d.v_out, 16) || !aligned(d.block_table, 4) ||
+      !aligned(d.starts, 4) || !aligned(d.lengths, 4) || !aligned(d.offsets, 4))
     return refuse(B200_E_ALIGN);
   if (device_info().sm_count == 0) return refuse(B200_E_DEVICE);
   ReadParams p{};
-  p.cache = device_cache(cache);
-  p.table = Table{block_table, table_stride, static_cast<int32_t>(table_width)};
-  p.k_out = k_out;
-  p.v_out = v_out;
-  p.starts = starts;
-  p.lengths = lengths;
-  p.offsets = offsets;
-  p.rows = rows;
-  p.batch = static_cast<int32_t>(batch);
+  p.cache = device_cache(&d.cache);
+  p.table = Table{d.block_table, d.table_stride, static_cast<int32_t>(d.table_width)};
+  p.k_out = d.k_out;
+  p.v_out = d.v_out;
+  p.starts = d.starts;
+  p.lengths = d.lengths;
+  p.offsets = d.offsets;
+  p.rows = d.rows;
+  p.batch = static_cast<int32_t>(d.batch);
   p.status = kernel_status_word();
   // two partial blocks a sequence at most, and the rows behind the last sequence
-  const int64_t pieces = rows / cache->block_tokens + 2 * batch + 1;
-  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(cache->heads), 2);
-  const unsigned threads = static_cast<unsigned>(cache->block_tokens / 4 * (cache->dim / 8));
+  const int64_t pieces = d.rows / d.cache.block_tokens + 2 * d.batch + 1;
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(d.cache.heads), 2);
+  const unsigned threads = static_cast<unsigned>(d.cache.block_tokens / 4 * (d.cache.dim / 8));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == B200_F32)
+  if (d.dtype == B200_F32)
     kv_read_kernel<float><<<grid, threads, 0, s>>>(p);
   else
     kv_read_kernel<__nv_bfloat16><<<grid, threads, 0, s>>>(p);

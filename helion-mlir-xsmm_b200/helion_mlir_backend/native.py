@@ -11,6 +11,7 @@ gets an exception.
 
 from __future__ import annotations
 
+from collections.abc import Callable
 import contextlib
 import ctypes
 from ctypes import c_char_p
@@ -21,8 +22,10 @@ from ctypes import c_int64
 from ctypes import c_size_t
 from ctypes import c_uint64
 from ctypes import c_void_p
+import math
 import os
 from pathlib import Path
+import struct
 import threading
 
 import torch
@@ -173,6 +176,64 @@ class KvCacheDesc(ctypes.Structure):
     ]
 
 
+class KvAppendDesc(ctypes.Structure):
+    """``b200_kv_append_desc`` of include/b200ops.h."""
+
+    _fields_ = [
+        ("cache", KvCacheDesc),
+        ("dtype", c_int32),
+        ("reserved_", c_int32),
+        *((name, c_void_p) for name in ("k", "v")),
+        *((name, c_int64) for name in ("k_row", "k_head", "v_row", "v_head")),
+        *((name, c_void_p) for name in ("block_table", "lengths", "offsets")),
+        *((name, c_int64) for name in ("table_stride", "table_width", "batch", "rows")),
+    ]
+
+
+class KvReadDesc(ctypes.Structure):
+    """``b200_kv_read_desc`` of include/b200ops.h."""
+
+    _fields_ = [
+        ("cache", KvCacheDesc),
+        ("dtype", c_int32),
+        ("reserved_", c_int32),
+        *((name, c_void_p) for name in ("k_out", "v_out", "block_table", "starts", "lengths", "offsets")),
+        *((name, c_int64) for name in ("table_stride", "table_width", "batch", "rows")),
+    ]
+
+
+class CachedAttentionDesc(ctypes.Structure):
+    """``b200_cached_attention_desc`` of include/b200ops.h."""
+
+    _fields_ = [
+        ("cache", KvCacheDesc),
+        ("dtype", c_int32),
+        ("scale", c_float),
+        *((name, c_void_p) for name in ("q", "out")),
+        *((name, c_int64) for name in ("q_batch", "q_token", "q_head")),
+        *((name, c_void_p) for name in ("block_table", "lengths")),
+        *((name, c_int64) for name in ("table_stride", "table_width", "batch", "tokens", "heads")),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+_FORMATS = {c_int32: "i", c_int64: "q", c_float: "f", c_void_p: "Q"}
+
+
+def _format(kind: type[ctypes.Structure]) -> str:
+    return "".join(_format(t) if issubclass(t, ctypes.Structure) else _FORMATS[t] for _, t in kind._fields_)
+
+
+def packer(kind: type[ctypes.Structure]) -> Callable[..., bytes]:
+    """``packer(Desc)(values...)``: the bytes of a descriptor, fields in order (nested ones in line), NULL as 0. A fifth of
+    the time that filling a ctypes structure takes, which counts where a whole call takes ten microseconds;
+    the entry points that take such descriptors are declared with a plain pointer, which takes bytes too."""
+    layout = struct.Struct("@" + _format(kind))
+    assert layout.size == ctypes.sizeof(kind), kind
+    return layout.pack
+
+
 class Counters(ctypes.Structure):
     _fields_ = [
         ("launches", c_uint64),
@@ -195,24 +256,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p],
     ),
-    "b200_attention_packed": (c_int, [ctypes.POINTER(PackedAttentionDesc), c_void_p]),
-    "b200_kv_append": (
-        c_int,
-        [ctypes.POINTER(KvCacheDesc), c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
-         c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p],
-    ),
-    "b200_kv_read": (
-        c_int,
-        [ctypes.POINTER(KvCacheDesc), c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
-         c_int64, c_int64, c_void_p],
-    ),
-    "b200_attention_cached_workspace_bytes": (
-        c_size_t, [ctypes.POINTER(KvCacheDesc), c_int64, c_int64, c_int64, c_int64]),
-    "b200_attention_cached": (
-        c_int,
-        [ctypes.POINTER(KvCacheDesc), c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
-         c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p, c_size_t, c_void_p],
-    ),
+    "b200_attention_packed": (c_int, [c_void_p, c_void_p]),
+    "b200_kv_append": (c_int, [c_void_p, c_void_p]),
+    "b200_kv_read": (c_int, [c_void_p, c_void_p]),
+    "b200_attention_cached_workspace_bytes": (c_int64, [c_void_p]),
+    "b200_attention_cached": (c_int, [c_void_p, c_void_p]),
     "b200_pack": (
         c_int,
         [c_int32, c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p],
@@ -368,6 +416,8 @@ def stream_ptr(device: torch.device) -> int:
     return _raw_stream(index)
 
 
+_POOLED_BYTES = 4 * 1024 * 1024  # output_pool.MIN_BYTES, which imports this module
+
 _NO_SWITCH = contextlib.nullcontext()
 
 
@@ -393,6 +443,35 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
             raise ValueError(f"operands are on different devices: {device} and {t.device}")
     assert device is not None
     return device
+
+
+def raw_stream(index: int) -> int:
+    """:func:`stream_ptr` of a device by its index."""
+    return _raw_stream(index)
+
+
+def new_output(shape: tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """An uninitialised result: large ones from the output pool, small ones (which it never takes) without asking it."""
+    if math.prod(shape) * dtype.itemsize < _POOLED_BYTES:
+        return torch.empty(shape, dtype=dtype, device=device)
+    from . import output_pool
+
+    return output_pool.empty(tuple(shape), dtype=dtype, device=device)
+
+
+def index_of(*tensors: torch.Tensor | None) -> int:
+    """The index of the CUDA device that all operands are on, for calls that are made often (a tenth of the time of
+    :func:`require_cuda`, whose errors it raises)."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            index = -1
+    return index if index >= 0 else require_cuda(*tensors).index
+
+
+def on_index(index: int):
+    """Context in which the device of :func:`index_of` is current."""
+    return _NO_SWITCH if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def counters() -> dict[str, int]:

@@ -16,7 +16,6 @@ into one tensor, causal, several query heads to a key/value head.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -98,43 +97,42 @@ attention.explain = explain_attention  # type: ignore[attr-defined]
 _MAX_DIM = 256
 
 
-def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor) -> None:
+_PACK_PACKED = native.packer(native.PackedAttentionDesc)
+_DTYPES = {torch.float32: native.F32, torch.bfloat16: native.BF16}
+
+
+def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor) -> int:
+    """The element type's code, after the checks of the operands."""
+    shape, k_shape = q.shape, k.shape
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"attention_packed() expects [rows, heads, dim] operands, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape != v.shape or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+    if k_shape != v.shape or k_shape[2] != shape[2] or k_shape[1] == 0 or shape[1] == 0 or shape[1] % k_shape[1]:
         raise ValueError("attention_packed() operands do not match (the heads of q have to be a multiple of those of k and v): "
                          f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if not 1 <= q.shape[2] <= _MAX_DIM:
+    if not 1 <= shape[2] <= _MAX_DIM:
         raise ValueError(f"attention_packed() expects heads of 1 to {_MAX_DIM}, got {tuple(q.shape)}")
-    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.bfloat16, torch.float32):
+    code = _DTYPES.get(q.dtype)
+    if code is None or not q.dtype is k.dtype is v.dtype:
         raise ValueError(f"attention_packed() requires matching bf16/f32 operands, got {q.dtype}, {k.dtype}, {v.dtype}")
     for name, t in (("offsets", offsets), ("k_offsets", k_offsets)):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape != offsets.shape or t.shape[0] < 1 or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.shape != offsets.shape or t.shape[0] < 1 or not t.is_contiguous():
             raise ValueError(f"attention_packed() expects {name} as a contiguous int32 tensor [sequences + 1], got {t.dtype} {tuple(t.shape)}")
-    if k_offsets is offsets and k.shape[0] != q.shape[0]:
+    if k_offsets is offsets and k_shape[0] != shape[0]:
         raise ValueError(f"attention_packed() needs k_offsets where k has other rows than q: {tuple(q.shape)}, {tuple(k.shape)}")
+    return code
 
 
-def _tensor_core(q: Tensor, scale: float | None) -> bool:
+def _tensor_core(q: Tensor, scale: float) -> bool:
     """Whether the tcgen05 kernel takes these operands (else f32 tiles on the CUDA cores)."""
-    return q.dtype == torch.bfloat16 and q.shape[2] in _FUSED_DIMS and (scale is None or 0.0 < scale < math.inf)
+    return q.dtype is torch.bfloat16 and q.shape[2] in _FUSED_DIMS and scale > 0.0
 
 
 def _for_tma(t: Tensor) -> Tensor:
     """``t`` if a TMA descriptor can hold its strides, else a contiguous copy."""
     row, head, dim = t.stride()
-    if dim == 1 and row > 0 and head > 0 and row % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0:
+    if dim == 1 and row > 0 and head > 0 and not (row % 8 or head % 8 or t.data_ptr() % 16):
         return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def _packed_desc(q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, offsets: Tensor, k_offsets: Tensor, scale: float,
-                 causal: bool) -> native.PackedAttentionDesc:
-    rows, heads, dim = q.shape
-    return native.PackedAttentionDesc(
-        native.dtype_code(q.dtype), causal, q.data_ptr(), k.data_ptr(), v.data_ptr(), native.ptr(out), q.stride(0), q.stride(1),
-        k.stride(0), k.stride(1), v.stride(0), v.stride(1), rows, k.shape[0], offsets.shape[0] - 1, heads, k.shape[1], dim,
-        offsets.data_ptr(), k_offsets.data_ptr(), scale, 0)
 
 
 def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor | None = None,
@@ -152,25 +150,29 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
     The offsets are not read on the host: a captured call can be replayed with other lengths of the same total. Offsets
     that decrease or leave the tensors raise bit 256 of ``native.kernel_status()`` and leave their rows unwritten."""
     k_offsets = offsets if k_offsets is None else k_offsets
-    _check_packed(q, k, v, offsets, k_offsets)
-    device = native.require_cuda(q, k, v, offsets, k_offsets)
+    code = _check_packed(q, k, v, offsets, k_offsets)
+    index = native.index_of(q, k, v, offsets, k_offsets)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if _tensor_core(q, scale):
-        q, k, v = _for_tma(q), _for_tma(k), _for_tma(v)
-    else:
-        q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
-    with native.on_device(device):
-        out = output_pool.empty(tuple(q.shape), dtype=q.dtype, device=device)
-        desc = _packed_desc(q, k, v, out, offsets, k_offsets, scale, bool(causal))
-        code = native.module().b200_attention_packed(ctypes.byref(desc), native.stream_ptr(device))
-    native.check("b200_attention_packed", code)
+    with native.on_index(index):
+        if _tensor_core(q, scale):
+            q, k, v = _for_tma(q), _for_tma(k), _for_tma(v)
+        else:
+            q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
+        rows, heads, dim = q.shape
+        out = native.new_output(q.shape, q.dtype, q.device)
+        result = native.module().b200_attention_packed(
+            _PACK_PACKED(code, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *q.stride()[:2],
+                         *k.stride()[:2], *v.stride()[:2], rows, k.shape[0], offsets.shape[0] - 1, heads, k.shape[1], dim,
+                         offsets.data_ptr(), k_offsets.data_ptr(), scale, 0),
+            native.raw_stream(index))
+    native.check("b200_attention_packed", result)
     return out
 
 
 def _explain_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor | None = None,
                     scale: float | None = None, causal: bool = True) -> CallExplanation:
     _check_packed(q, k, v, offsets, offsets if k_offsets is None else k_offsets)
-    if _tensor_core(q, scale):
+    if _tensor_core(q, 1.0 if scale is None else scale):
         return CallExplanation(True, "packed_umma_kernel (tcgen05, two tiles of 128 queries x 128 keys per step, scores in TMEM)")
     return CallExplanation(True, "packed_simt_kernel (f32 tiles of 64 x 64)")
 

@@ -21,7 +21,6 @@ prefix back for ``attention_packed`` of a later chunk of the prompt.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple
 
@@ -29,7 +28,6 @@ import torch
 from torch import Tensor
 
 from helion_mlir_backend import native
-from helion_mlir_backend import output_pool
 from helion_mlir_backend.call_trace import CallExplanation
 
 BLOCK_TOKENS = (16, 32, 64)
@@ -59,10 +57,16 @@ def quantized_cache(blocks: int, heads: int, dim: int, block_tokens: int = 64, d
     )
 
 
-def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[native.KvCacheDesc, int, int]:
-    """The library's view of the cache, its heads and head size."""
+_PACK_APPEND = native.packer(native.KvAppendDesc)
+_PACK_READ = native.packer(native.KvReadDesc)
+_PACK_CACHED = native.packer(native.CachedAttentionDesc)
+_DTYPES = {torch.float32: native.F32, torch.bfloat16: native.BF16}
+
+
+def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[int, ...]:
+    """The fields of ``b200_kv_cache``, after the checks of the four tensors."""
     k_codes, v_codes, k_scales, v_scales = cache
-    if k_codes.dim() != 4 or v_codes.dim() != 4:
+    if k_codes.dim() != 4:
         raise ValueError(f"{name}() expects codes [blocks, heads, tokens, dim] and [blocks, heads, dim, tokens], "
                          f"got {tuple(k_codes.shape)} and {tuple(v_codes.shape)}")
     blocks, heads, tokens, dim = k_codes.shape
@@ -71,33 +75,37 @@ def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[
     if v_codes.shape != (blocks, heads, dim, tokens) or k_scales.shape != (blocks, heads) or v_scales.shape != (blocks, heads):
         raise ValueError(f"{name}() cache tensors do not match: codes {tuple(k_codes.shape)} and {tuple(v_codes.shape)}, "
                          f"scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}")
-    if (k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or k_scales.dtype != torch.float32
-            or v_scales.dtype != torch.float32):
+    if not (k_codes.dtype is v_codes.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32):
         raise ValueError(f"{name}() expects int8 codes and f32 scales, got {k_codes.dtype}, {v_codes.dtype}, {k_scales.dtype}, {v_scales.dtype}")
     if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
         raise ValueError(f"{name}() expects contiguous cache tensors")
-    return native.KvCacheDesc(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), blocks, heads,
-                              dim, tokens, 0), heads, dim
+    return k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), blocks, heads, dim, tokens, 0
 
 
-def _indices(name: str, what: str, t: Tensor, shape: tuple[int, ...]) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name}() expects {what} as a contiguous int32 tensor {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+def _indices(name: str, what: str, t: Tensor, count: int) -> int:
+    """The address of an int32 vector of ``count`` values."""
+    if t.dtype is not torch.int32 or t.shape != (count,) or not t.is_contiguous():
+        raise ValueError(f"{name}() expects {what} as a contiguous int32 tensor [{count}], got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def _table(name: str, table: Tensor) -> tuple[int, int, int]:
     """Sequences, row stride and width of a block table."""
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    if table.dtype is not torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"{name}() expects block_table as an int32 tensor [sequences, blocks] with contiguous rows, "
                          f"got {table.dtype} {tuple(table.shape)}")
     batch, width = table.shape
-    return batch, max(table.stride(0), width), width
+    stride = table.stride(0)
+    if batch > 1 and stride < width:
+        raise ValueError(f"{name}() expects block_table rows that do not overlap, got strides {table.stride()}")
+    return batch, stride, width
 
 
 def _aligned_rows(t: Tensor) -> Tensor:
-    """``t`` if its rows can be read as 16-byte vectors, else a contiguous copy."""
+    """``t`` ``[rows, heads, dim]`` if its rows can be read as 16-byte vectors, else a contiguous copy."""
+    row, head, dim = t.stride()
     step = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:-1]):
+    if dim == 1 and not (row % step or head % step or t.data_ptr() % 16):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -114,29 +122,29 @@ def cache_append(cache: tuple[Tensor, Tensor, Tensor, Tensor], k: Tensor, v: Ten
     shrinks, and when it grows the older codes become ``rint(code * old / new)``. Codes are rounded to the nearest, ties to
     even. A value that is not finite makes the scale NaN. ``lengths`` is left as it is (the caller adds the
     new tokens); the blocks have to be in the table already. No block may belong to two of the sequences that are written."""
-    desc, heads, dim = _describe(cache, "cache_append")
+    fields = _describe(cache, "cache_append")
+    heads, dim = fields[5], fields[6]
     batch, stride, width = _table("cache_append", block_table)
-    if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float32):
+    code = _DTYPES.get(k.dtype)
+    if code is None or k.dtype is not v.dtype or k.shape != v.shape:
         raise ValueError(f"cache_append() expects matching bf16/f32 k and v, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    if tuple(k.shape[-2:]) != (heads, dim) or k.dim() not in ((3,) if offsets is not None else (3, 4)):
-        raise ValueError(f"cache_append() expects k and v [rows, {heads}, {dim}] (or [sequences, new, {heads}, {dim}] without "
-                         f"offsets), got {tuple(k.shape)}")
-    _indices("cache_append", "lengths", lengths, (batch,))
-    if offsets is not None:
-        _indices("cache_append", "offsets", offsets, (batch + 1,))
-    elif k.shape[0] != batch:
-        raise ValueError(f"cache_append() expects k and v of {batch} sequences, got {tuple(k.shape)}")
-    device = native.require_cuda(*cache, k, v, block_table, lengths, offsets)
-    if k.dim() == 4:
+    if k.dim() == 4 and offsets is None and k.shape[0] == batch:
         k, v = k.flatten(0, 1), v.flatten(0, 1)
-    k, v = _aligned_rows(k), _aligned_rows(v)
-    with native.on_device(device):
-        code = native.module().b200_kv_append(
-            ctypes.byref(desc), native.dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
-            v.stride(1), block_table.data_ptr(), stride, width, lengths.data_ptr(), native.ptr(offsets), batch, k.shape[0],
-            native.stream_ptr(device),
-        )
-    native.check("b200_kv_append", code)
+    elif k.dim() != 3 or (offsets is None and k.shape[0] != batch):
+        raise ValueError(f"cache_append() expects k and v [rows, heads, dim] with offsets, or [sequences, heads, dim] or [sequences, new, "
+                         f"heads, dim] of {batch} sequences without, got {tuple(k.shape)}")
+    if k.shape[1] != heads or k.shape[2] != dim:
+        raise ValueError(f"cache_append() expects k and v of {heads} heads of {dim}, got {tuple(k.shape)}")
+    lengths_ptr = _indices("cache_append", "lengths", lengths, batch)
+    offsets_ptr = 0 if offsets is None else _indices("cache_append", "offsets", offsets, batch + 1)
+    index = native.index_of(k, v, *cache, block_table, lengths, offsets)
+    with native.on_index(index):
+        k, v = _aligned_rows(k), _aligned_rows(v)
+        result = native.module().b200_kv_append(
+            _PACK_APPEND(*fields, code, 0, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                         block_table.data_ptr(), lengths_ptr, offsets_ptr, stride, width, batch, k.shape[0]),
+            native.raw_stream(index))
+    native.check("b200_kv_append", result)
 
 
 def cache_read(cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, starts: Tensor, lengths: Tensor,
@@ -144,31 +152,34 @@ def cache_read(cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor
     """Positions ``starts[b] ...`` of each sequence as values: ``(k, v)``, each ``[rows, heads, dim]`` in ``dtype`` (bf16 or f32),
     packed: sequence ``b`` fills the rows ``offsets[b] .. offsets[b + 1]``. Positions that the sequence does not
     hold (at or beyond ``lengths[b]``) and rows behind the last sequence are zeros."""
-    desc, heads, dim = _describe(cache, "cache_read")
+    fields = _describe(cache, "cache_read")
+    heads, dim = fields[5], fields[6]
     batch, stride, width = _table("cache_read", block_table)
-    if dtype not in (torch.bfloat16, torch.float32) or rows < 0:
+    code = _DTYPES.get(dtype)
+    if code is None or rows < 0:
         raise ValueError(f"cache_read() expects rows >= 0 and dtype bf16/f32, got {rows} and {dtype}")
-    _indices("cache_read", "starts", starts, (batch,))
-    _indices("cache_read", "lengths", lengths, (batch,))
-    _indices("cache_read", "offsets", offsets, (batch + 1,))
-    device = native.require_cuda(*cache, block_table, starts, lengths, offsets)
-    with native.on_device(device):
-        k = output_pool.empty((rows, heads, dim), dtype=dtype, device=device)
-        v = output_pool.empty((rows, heads, dim), dtype=dtype, device=device)
-        code = native.module().b200_kv_read(
-            ctypes.byref(desc), native.dtype_code(dtype), k.data_ptr(), v.data_ptr(), block_table.data_ptr(), stride, width,
-            starts.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), batch, rows, native.stream_ptr(device),
-        )
-    native.check("b200_kv_read", code)
+    starts_ptr, lengths_ptr = _indices("cache_read", "starts", starts, batch), _indices("cache_read", "lengths", lengths, batch)
+    offsets_ptr = _indices("cache_read", "offsets", offsets, batch + 1)
+    index = native.index_of(*cache, block_table, starts, lengths, offsets)
+    with native.on_index(index):
+        k, v = native.new_output((2, rows, heads, dim), dtype, block_table.device).unbind(0)
+        result = native.module().b200_kv_read(
+            _PACK_READ(*fields, code, 0, k.data_ptr(), v.data_ptr(), block_table.data_ptr(), starts_ptr, lengths_ptr, offsets_ptr,
+                       stride, width, batch, rows),
+            native.raw_stream(index))
+    native.check("b200_kv_read", result)
     return k, v
 
 
-def _check_cached(q: Tensor, heads: int, dim: int, batch: int) -> None:
-    if q.dtype not in (torch.bfloat16, torch.float32) or q.dim() not in (3, 4) or q.shape[-1] != dim or q.shape[-2] % heads:
+def _check_cached(q: Tensor, heads: int, dim: int, batch: int) -> tuple[int, int, int]:
+    """Element type, tokens and query heads."""
+    code, rank = _DTYPES.get(q.dtype), q.dim()
+    if code is None or rank not in (3, 4) or q.shape[-1] != dim or q.shape[-2] % heads:
         raise ValueError(f"attention_cached() expects bf16/f32 q [sequences, heads, {dim}] or [sequences, tokens, heads, {dim}] with "
                          f"heads a multiple of {heads}, got {q.dtype} {tuple(q.shape)}")
     if q.shape[0] != batch or q.shape[-2] == 0:
         raise ValueError(f"attention_cached() expects q of {batch} sequences and at least one head, got {tuple(q.shape)}")
+    return code, 1 if rank == 3 else q.shape[1], q.shape[-2]
 
 
 def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, lengths: Tensor,
@@ -179,35 +190,35 @@ def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], bl
     ``tokens`` of the ``lengths[b]`` positions of sequence ``b``, which :func:`cache_append` has written already;
     token ``i`` sees the positions below ``lengths[b] - tokens + i + 1`` (a row that sees none is zeros). Query head ``h`` reads
     key/value head ``h // (heads // kv_heads)``. Result in ``q``'s type and shape."""
-    desc, heads, dim = _describe(cache, "attention_cached")
+    fields = _describe(cache, "attention_cached")
+    dim = fields[6]
     batch, stride, width = _table("attention_cached", block_table)
-    _check_cached(q, heads, dim, batch)
-    _indices("attention_cached", "lengths", lengths, (batch,))
-    device = native.require_cuda(q, *cache, block_table, lengths)
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if q.stride(-1) != 1:
-        q = q.contiguous()
-    tokens = 1 if q.dim() == 3 else q.shape[1]
+    code, tokens, heads = _check_cached(q, fields[5], dim, batch)
+    lengths_ptr = _indices("attention_cached", "lengths", lengths, batch)
+    index = native.index_of(q, *cache, block_table, lengths)
     lib = native.module()
-    with native.on_device(device):
-        out = output_pool.empty(tuple(q.shape), dtype=q.dtype, device=device)
-        need = lib.b200_attention_cached_workspace_bytes(ctypes.byref(desc), batch, tokens, q.shape[-2], width)
-        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        code = lib.b200_attention_cached(
-            ctypes.byref(desc), native.dtype_code(q.dtype), q.data_ptr(), q.stride(0), q.stride(1) if tokens > 1 else 0,
-            q.stride(-2), out.data_ptr(), block_table.data_ptr(), stride, width, lengths.data_ptr(), batch, tokens, q.shape[-2],
-            scale, native.ptr(workspace), need, native.stream_ptr(device),
-        )
-    native.check("b200_attention_cached", code)
+    with native.on_index(index):
+        if q.stride(-1) != 1:
+            q = q.contiguous()
+        out = native.new_output(q.shape, q.dtype, q.device)
+
+        def desc(workspace: int, held: int) -> bytes:
+            return _PACK_CACHED(*fields, code, 1.0 / math.sqrt(dim) if scale is None else scale, q.data_ptr(), out.data_ptr(),
+                                q.stride(0), q.stride(1) if tokens > 1 else 0, q.stride(-2), block_table.data_ptr(), lengths_ptr,
+                                stride, width, batch, tokens, heads, workspace, held)
+
+        need = lib.b200_attention_cached_workspace_bytes(desc(0, 0))
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        result = lib.b200_attention_cached(desc(workspace.data_ptr(), need), native.raw_stream(index))
+    native.check("b200_attention_cached", result)
     return out
 
 
 def _explain_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, lengths: Tensor,
                     scale: float | None = None) -> CallExplanation:
-    _, heads, dim = _describe(cache, "attention_cached")
-    _check_cached(q, heads, dim, _table("attention_cached", block_table)[0])
-    tokens = 1 if q.dim() == 3 else q.shape[1]
-    rows = tokens * (q.shape[-2] // heads)
+    fields = _describe(cache, "attention_cached")
+    _, tokens, heads = _check_cached(q, fields[5], fields[6], _table("attention_cached", block_table)[0])
+    rows = tokens * (heads // fields[5])
     return CallExplanation(True, f"cached_kernel (mma f16, {8 if rows <= 8 else 16} query rows a tile, {rows} rows a head) + cached_join_kernel")
 
 

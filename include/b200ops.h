@@ -218,28 +218,47 @@ typedef struct b200_kv_cache {
  * ties to even; where s grew, older codes become code * s_old / s, rounded the same way. A value
  * that is not finite makes s NaN (for the rest of the block's use). `lengths` is not changed.
  * No block may be written for two sequences in one call. */
-int b200_kv_append(const b200_kv_cache* cache, int32_t dtype, const void* k, const void* v, int64_t k_row, int64_t k_head,
-                   int64_t v_row, int64_t v_head, const int32_t* block_table, int64_t table_stride, int64_t table_width,
-                   const int32_t* lengths, const int32_t* offsets, int64_t batch, int64_t rows, void* stream);
+typedef struct b200_kv_append_desc {
+  b200_kv_cache cache;
+  int32_t dtype, reserved_;
+  const void *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  const int32_t *block_table, *lengths, *offsets;
+  int64_t table_stride, table_width, batch, rows;
+} b200_kv_append_desc;
+int b200_kv_append(const b200_kv_append_desc* desc, void* stream);
 
 /* Reads positions starts[b] ... of each sequence back as values: k_out, v_out [rows][heads][dim]
  * contiguous (16-byte aligned); sequence b fills the rows [offsets[b], offsets[b+1]).
  * Positions at or beyond lengths[b] and the rows behind the last sequence are zeros. */
-int b200_kv_read(const b200_kv_cache* cache, int32_t dtype, void* k_out, void* v_out, const int32_t* block_table,
-                 int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths,
-                 const int32_t* offsets, int64_t batch, int64_t rows, void* stream);
+typedef struct b200_kv_read_desc {
+  b200_kv_cache cache;
+  int32_t dtype, reserved_;
+  void *k_out, *v_out;
+  const int32_t *block_table, *starts, *lengths, *offsets;
+  int64_t table_stride, table_width, batch, rows;
+} b200_kv_read_desc;
+int b200_kv_read(const b200_kv_read_desc* desc, void* stream);
 
 /* Attention of the last `tokens` positions of each sequence (lengths[b] positions, these
  * included) over the cache: q [batch][tokens][heads][dim], out the same, contiguous;
  * token i sees the positions below lengths[b] - tokens + i + 1, none: zeros. Sums and the
- * softmax are f32. The workspace (16-byte aligned, of the size the query says) holds partial
- * results during the call; nothing in it has to be kept or cleared. */
-size_t b200_attention_cached_workspace_bytes(const b200_kv_cache* cache, int64_t batch, int64_t tokens, int64_t heads,
-                                             int64_t table_width);
-int b200_attention_cached(const b200_kv_cache* cache, int32_t dtype, const void* q, int64_t q_batch, int64_t q_token,
-                          int64_t q_head, void* out, const int32_t* block_table, int64_t table_stride, int64_t table_width,
-                          const int32_t* lengths, int64_t batch, int64_t tokens, int64_t heads, float scale,
-                          void* workspace, size_t workspace_bytes, void* stream);
+ * softmax are f32. The workspace (16-byte aligned, of the size the query says for the same
+ * descriptor on the same device) holds partial results during the call; nothing in it has to be kept or cleared. */
+typedef struct b200_cached_attention_desc {
+  b200_kv_cache cache;
+  int32_t dtype;
+  float scale;
+  const void* q;
+  void* out;
+  int64_t q_batch, q_token, q_head;
+  const int32_t *block_table, *lengths;
+  int64_t table_stride, table_width, batch, tokens, heads;
+  void* workspace;
+  int64_t workspace_bytes;
+} b200_cached_attention_desc;
+int64_t b200_attention_cached_workspace_bytes(const b200_cached_attention_desc* desc);
+int b200_attention_cached(const b200_cached_attention_desc* desc, void* stream);
 
 /* Layout conversions (bit-exact copies with zero fill). `kind`: */
 enum {

@@ -75,7 +75,7 @@ def test_cache_refusals() -> None:
         ops.cache_append(cache, k, k, table, ints(0, 0))
     with pytest.raises(ValueError, match="offsets"):
         ops.cache_append(cache, k, k, table, lengths, ints(0, 1, 2))
-    with pytest.raises(ValueError, match="rows"):
+    with pytest.raises(ValueError, match="heads, dim"):
         ops.cache_append(cache, k[:, None], k[:, None], table, lengths, ints(0, 1, 2, 3))
     with pytest.raises(ValueError, match="cache_read"):
         ops.cache_read(cache, table, lengths, lengths, ints(0, 1, 2, 3), 3, torch.float16)
@@ -117,16 +117,23 @@ def test_c_abi_refusals() -> None:
         fields.update(change)
         return native.KvCacheDesc(**fields)
 
-    def append(c, dtype=native.BF16, k=at, v=at, strides=(128, 64, 128, 64), stride=2, width=2, lengths=at, offsets=at, batch=2,
-               rows=2):
-        return lib.b200_kv_append(ctypes.byref(c), dtype, k, v, *strides, at, stride, width, lengths, offsets, batch, rows, None)
+    def append(c, **change):
+        fields = dict(cache=c, dtype=native.BF16, k=at, v=at, k_row=128, k_head=64, v_row=128, v_head=64, block_table=at, lengths=at,
+                      offsets=at, table_stride=2, table_width=2, batch=2, rows=2)
+        fields.update(change)
+        return lib.b200_kv_append(ctypes.byref(native.KvAppendDesc(**fields)), None)
 
-    def read(c, dtype=native.BF16, out=at, offsets=at, stride=2, batch=2, rows=2):
-        return lib.b200_kv_read(ctypes.byref(c), dtype, out, out, at, stride, 2, at, at, offsets, batch, rows, None)
+    def read(c, **change):
+        fields = dict(cache=c, dtype=native.BF16, k_out=at, v_out=at, block_table=at, starts=at, lengths=at, offsets=at, table_stride=2,
+                      table_width=2, batch=2, rows=2)
+        fields.update(change)
+        return lib.b200_kv_read(ctypes.byref(native.KvReadDesc(**fields)), None)
 
-    def attend(c, dtype=native.BF16, q=at, heads=4, batch=2, tokens=1, scale=1.0, lengths=at, stride=2):
-        return lib.b200_attention_cached(ctypes.byref(c), dtype, q, 256, 256, 64, at, at, stride, 2, lengths, batch, tokens, heads,
-                                         scale, None, 0, None)
+    def attend(c, **change):
+        fields = dict(cache=c, dtype=native.BF16, scale=1.0, q=at, out=at, q_batch=256, q_token=256, q_head=64, block_table=at, lengths=at,
+                      table_stride=2, table_width=2, batch=2, tokens=1, heads=4)
+        fields.update(change)
+        return lib.b200_attention_cached(ctypes.byref(native.CachedAttentionDesc(**fields)), None)
 
     for call in (append, read, attend):
         assert call(cache(), dtype=5) == 1
@@ -134,22 +141,47 @@ def test_c_abi_refusals() -> None:
             assert call(cache(**change)) == 2, change
         assert call(cache(k_codes=None)) == 6 and call(cache(v_scales=None)) == 6
         assert call(cache(k_codes=at + 8)) == 4
-        assert call(cache(), stride=1) == 3
+        assert call(cache(), table_stride=1) == 3 and call(cache(), table_width=-1) == 3
         assert call(cache(), batch=-1) == 2
-    assert append(cache(), offsets=None, batch=2, rows=3) == 2
-    assert append(cache(), strides=(129, 64, 128, 64)) == 3 and append(cache(), k=at + 2) == 4
+        assert call(cache(), block_table=at + 2) == 4
+    assert append(cache(), offsets=None, rows=3) == 2
+    assert append(cache(), k_row=129) == 3 and append(cache(), k=at + 2) == 4
     assert append(cache(), k=None) == 6 and append(cache(), lengths=None) == 6
     assert append(cache(), batch=0) == 0 and append(cache(), rows=0) == 0
-    assert read(cache(), out=None) == 6 and read(cache(), offsets=None) == 6 and read(cache(), out=at + 8) == 4
+    assert read(cache(), k_out=None) == 6 and read(cache(), offsets=None) == 6 and read(cache(), v_out=at + 8) == 4
     assert read(cache(), rows=0) == 0
     assert attend(cache(), heads=3) == 2 and attend(cache(), tokens=-1) == 2 and attend(cache(), scale=float("nan")) == 7
     assert attend(cache(), q=None) == 6 and attend(cache(), batch=0) == 0 and attend(cache(), tokens=0) == 0
-    for fn in ("b200_kv_append", "b200_kv_read", "b200_attention_cached"):
-        args = [0] * (len(native.SIGNATURES[fn][1]) - 1)
-        assert getattr(lib, fn)(None, *args) == 6, fn
+    for fn in (lib.b200_kv_append, lib.b200_kv_read, lib.b200_attention_cached):
+        assert fn(None, None) == 6
+    assert lib.b200_attention_cached_workspace_bytes(None) == 0
 
 
-@pytest.mark.parametrize("name,struct", [("b200_packed_attention_desc", native.PackedAttentionDesc), ("b200_kv_cache", native.KvCacheDesc)])
+_STRUCTS = [
+    ("b200_packed_attention_desc", native.PackedAttentionDesc), ("b200_kv_cache", native.KvCacheDesc),
+    ("b200_kv_append_desc", native.KvAppendDesc), ("b200_kv_read_desc", native.KvReadDesc),
+    ("b200_cached_attention_desc", native.CachedAttentionDesc),
+]
+
+
+def test_packed_descriptors_are_the_structures() -> None:
+    """The bytes that the operators pass are those of the ctypes mirror with the same values."""
+    for _, kind in _STRUCTS:
+        def fill(structure, start: int) -> list[int]:
+            values = []
+            for name, field in structure._fields_:
+                if issubclass(field, ctypes.Structure):
+                    values += fill(getattr(structure, name), start + len(values))
+                else:
+                    values.append(start + len(values) + 1)
+                    setattr(structure, name, values[-1])
+            return values
+
+        structure = kind()
+        assert native.packer(kind)(*fill(structure, 0)) == bytes(structure)
+
+
+@pytest.mark.parametrize("name,struct", _STRUCTS)
 def test_struct_layouts_match_the_header(name: str, struct) -> None:
     text = (Path(__file__).resolve().parent.parent / "include" / "b200ops.h").read_text()
     body = text[text.index(f"typedef struct {name} {{") + len(f"typedef struct {name} {{") : text.index(f"}} {name};")]
