@@ -15,52 +15,89 @@ namespace {
 constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100: rint's test products stay normal numbers
 constexpr uint32_t kInfBits = 0x7f800000u;
 
-// rint(x / s) to the last tie: a first guess from the reciprocal, which is off by at most one,
-// moved by the exact signs of x - (r +- 1/2) s (one rounding of an exact product and sum: the
-// sign is right, and zero is a tie, which goes to the even neighbour).
-__device__ __forceinline__ int quotient_code(float x, float s, float inv) {
-  float r = rintf(x * inv);
+// Conversions by the bits of 1.5 * 2^23 + n: cvt and rint run at a quarter of the rate of the FMA pipe and set the time
+// of both kernels otherwise (a write of prompts 55 us in place of 20).
+constexpr float kWhole = 12582912.f;
+// x / s to the nearest, as the bits of kWhole + code (the low byte is the code): `inv` is within 2^-23 of 1 / s, so the result can
+// only be wrong next to a tie, which `near_tie` tells from the remainder.
+__device__ __forceinline__ float quotient(float x, float s, float inv, bool& near_tie) {
+  const float shifted = fmaf(x, inv, kWhole);
+  const float rest = fmaf(-(shifted - kWhole), s, x);
+  near_tie |= fabsf(rest) > 0.4999f * s;
+  return shifted;
+}
+// rint(x / s), ties to even: the guess moved by the exact signs of x - (r +- 1/2) s (one rounding of an exact product and
+// sum: the sign is right, and zero is a tie).
+__device__ __forceinline__ float quotient_at_tie(float x, float s, float shifted) {
+  float r = shifted - kWhole;
   const float over = fmaf(-(r + 0.5f), s, x), under = fmaf(-(r - 0.5f), s, x);
   const bool odd = static_cast<int>(r) & 1;
   if (over > 0.f || (over == 0.f && odd)) r += 1.f;
   if (under < 0.f || (under == 0.f && odd)) r -= 1.f;
-  return static_cast<int>(r);
+  return r + kWhole;
 }
-// rint(code * old / s): both sides of each comparison are exact in f64 (at most 33 bits).
-__device__ __forceinline__ int rescaled_code(int code, float old, float s) {
-  const double x = static_cast<double>(code) * old, step = s;
-  double r = rint(x / step);
-  const bool odd = static_cast<int>(r) & 1;
-  const double over = x - (r + 0.5) * step, under = x - (r - 0.5) * step;
-  if (over > 0. || (over == 0. && odd)) r += 1.;
-  if (under < 0. || (under == 0. && odd)) r -= 1.;
-  return static_cast<int>(r);
+// rint(code * old / s), old <= s: as above, with both sides of the comparison exact in f64 (32 bits at most), which is
+// looked at only where the quotient is near a tie.
+__device__ __forceinline__ float code_value(uint32_t word, int i) {  // of byte i: 2^23 + 128 + code, less 2^23 + 128
+  return __uint_as_float(__byte_perm(word ^ 0x80808080u, 0x4B000000u, 0x7440 + i)) - 8388736.f;
+}
+__device__ __forceinline__ float rescaled(float code, float old, float s, float ratio) {
+  const float q = code * ratio, shifted = q + kWhole;
+  if (fabsf(fabsf(q - (shifted - kWhole)) - 0.5f) > 1e-3f) return shifted;
+  const double low = floor(static_cast<double>(q));
+  const double off = static_cast<double>(code) * old - (low + 0.5) * s;  // above or below the tie that is near
+  const bool odd = static_cast<int>(low) & 1;
+  return static_cast<float>(low) + (off > 0. || (off == 0. && odd) ? 1.f : 0.f) + kWhole;
+}
+// Byte `i` of `word` replaced by the low byte of `code`'s bits.
+__device__ __forceinline__ uint32_t with_code(uint32_t word, int i, float code) {
+  return __byte_perm(word, __float_as_uint(code), i == 0 ? 0x3214 : (i == 1 ? 0x3240 : (i == 2 ? 0x3410 : 0x4210)));
 }
 
-__device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {
-  return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | static_cast<uint32_t>(d & 255) << 24;
-}
-__device__ __forceinline__ int code_at(uint32_t word, int i) { return static_cast<int8_t>(word >> (8 * i)); }
-
-// 8 consecutive values.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const uint4 lo = ld_plain16(p), hi = ld_plain16(p + 4);
-  float a[4], b[4];
-  unpack16(lo, a);
-  unpack16(hi, b);
+// 8 consecutive values as they lie in memory.
+template <typename T>
+struct Eight {
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = a[i];
-    v[4 + i] = b[i];
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) raw[i] = ld_stream16(p + i * Elem<T>::kVec);
   }
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) { unpack16(ld_plain16(p), v); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+  }
+  // The largest magnitude's bits as f32 (infinities above all numbers, NaN above them).
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (sizeof(T) == 4)
+          m = max(m, w[e] & 0x7fffffffu);
+        else
+          m = __vmaxu2(m, w[e] & 0x7fff7fffu);
+      }
+    }
+    return sizeof(T) == 4 ? m : max(m << 16, m & 0xffff0000u);
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    float part[Elem<T>::kVec];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) {
+      unpack16(raw[i], part);
+#pragma unroll
+      for (int e = 0; e < Elem<T>::kVec; ++e) v[i * Elem<T>::kVec + e] = part[e];
+    }
+  }
+};
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-  *reinterpret_cast<uint4*>(p) = pack16(a);
-  *reinterpret_cast<uint4*>(p + 4) = pack16(b);
+  st_stream16(p, pack16(a));
+  st_stream16(p + 4, pack16(b));
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) { *reinterpret_cast<uint4*>(p) = pack16(v); }
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) { st_stream16(p, pack16(v)); }
 
 struct AppendParams {
   Cache cache;
@@ -70,17 +107,18 @@ struct AppendParams {
   const int32_t *lengths, *offsets;      // lengths before; offsets NULL: `each` new tokens per sequence
   int64_t rows;
   int32_t batch, each;
+  int32_t heads_each;  // heads that one CTA takes, one after the other
   int32_t* status;
 };
 
 // A thread holds 8 values of each of 4 consecutive tokens. Threads of a warp go along the head first
 // for K (8 code bytes of a token next to each other) and along the tokens first for V (4 codes of a
-// channel in one word, the words of a channel next to each other), so both leave in whole sectors.
-template <typename T>
-__global__ void kv_append_kernel(const AppendParams p) {
+// channel in one word, the words of a channel next to each other), so both leave in whole sectors. Where there is
+// work for all SMs a CTA goes over several heads, with the next head's values on their way while it reduces and
+// stores: finding its block (four dependent loads) is done once, and memory is not idle in between.
+template <typename T, bool is_v>
+__device__ __forceinline__ void append_block(const AppendParams& p) {
   const Cache& c = p.cache;
-  const bool is_v = blockIdx.z;
-  const int head = blockIdx.y;
   auto new_rows = [&](int32_t b) {
     if (p.offsets) return rows_of(p.offsets, b, p.rows, p.status);
     return Rows{static_cast<int64_t>(b) * p.each, p.each};
@@ -100,86 +138,127 @@ __global__ void kv_append_kernel(const AppendParams p) {
   const int64_t start = page << c.token_bits;
   const int first = static_cast<int>(max(length, start) - start);  // slots [first, stop) are new
   const int stop = static_cast<int>(min(length + rows.count, start + c.tokens) - start);
-  const int64_t row = rows.begin + start - length;  // of slot 0
 
   const int parts = c.dim / 8, groups = c.tokens / 4;
   const int part = is_v ? threadIdx.x / groups : threadIdx.x % parts;
   const int slot0 = 4 * (is_v ? threadIdx.x % groups : threadIdx.x / parts);
-  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head) + part * 8;
-  const int64_t step = is_v ? p.v_row : p.k_row;
-  float x[4][8];
-  uint32_t largest = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int slot = slot0 + j;
-    if (slot >= first && slot < stop) {
-      load8(src + (row + slot) * step, x[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(x[j][i]) & 0x7fffffffu);  // NaN above infinity
-  }
-  __shared__ uint32_t warp_largest[8];
-  __shared__ float old_scale;
-  float* scale = (is_v ? c.v_scales : c.k_scales) + block * c.heads + head;
-  largest = __reduce_max_sync(0xffffffffu, largest);
-  if ((threadIdx.x & 31) == 0) warp_largest[threadIdx.x >> 5] = largest;
-  if (threadIdx.x == 0) old_scale = first > 0 ? *scale : 0.f;
-  __syncthreads();
-  largest = warp_largest[0];
-  for (unsigned w = 1; w < blockDim.x / 32; ++w) largest = max(largest, warp_largest[w]);
-  const float before = old_scale;
-  float s = fmaxf(fmaxf(__fdiv_rn(__uint_as_float(largest), 127.f), kSmallestScale), before);
-  const bool finite = largest < kInfBits && before == before;
-  if (!finite) s = __uint_as_float(0x7fc00000u);
-  if (threadIdx.x == 0 && !(s == before)) *scale = s;
+  const int64_t step = is_v ? p.v_row : p.k_row, head_step = is_v ? p.v_head : p.k_head;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + part * 8 + (rows.begin + start - length) * step;
+  auto is_new = [&](int j) { return slot0 + j >= first && slot0 + j < stop; };
+  const bool any_new = slot0 + 4 > first && slot0 < stop, all_new = slot0 >= first && slot0 + 4 <= stop;
+  const bool any_old = slot0 < first;
 
-  int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
-  if (first > 0 && finite && s > before) {
-    // The older tokens' codes follow the scale: rare (a running maximum over a block's tokens).
-    for (int i = threadIdx.x; i < c.dim * first; i += blockDim.x) {
-      int8_t* at = codes + (is_v ? (i / first) * c.tokens + i % first : i);
-      *at = static_cast<int8_t>(rescaled_code(*at, before, s));
-    }
-  }
-  const float inv = __frcp_rn(s);
-  uint32_t word[8];  // K: two words of each token; V: one word of each channel
-#pragma unroll
-  for (int i = 0; i < 8; ++i) word[i] = 0;
-  if (finite) {
+  __shared__ uint32_t warp_largest[2][8];
+  const int head0 = blockIdx.y * p.heads_each, head_end = min(head0 + p.heads_each, c.heads);
+  Eight<T> next[4];
+  float next_scale = 0.f;
+  auto fetch = [&](int head) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      int code[8];
+      if (is_new(j))
+        next[j].load(src + head * head_step + (slot0 + j) * step);
+      else
+        next[j].clear();
+    }
+    if (first > 0) next_scale = (is_v ? c.v_scales : c.k_scales)[block * c.heads + head];
+  };
+  fetch(head0);
+  for (int head = head0; head < head_end; ++head) {
+    Eight<T> here[4];
+    uint32_t largest = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) code[i] = quotient_code(x[j][i], s, inv);
+    for (int j = 0; j < 4; ++j) {
+      here[j] = next[j];
+      largest = max(largest, here[j].largest());
+    }
+    const float before = next_scale;
+    if (head + 1 < head_end) fetch(head + 1);
+    int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
+    // K: two words of each token; V: one word of each channel. What is there counts only where older
+    // tokens or bytes of other slots share a word.
+    uint32_t word[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[i] = 0;
+    if (is_v ? (any_old || any_new) && !all_new : any_old) {
       if (is_v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word[i] |= static_cast<uint32_t>(code[i] & 255) << (8 * j);
+        for (int i = 0; i < 8; ++i) word[i] = *reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0);
       } else {
-        word[2 * j] = pack_codes(code[0], code[1], code[2], code[3]);
-        word[2 * j + 1] = pack_codes(code[4], code[5], code[6], code[7]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint2 w = *reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8);
+          word[2 * j] = w.x;
+          word[2 * j + 1] = w.y;
+        }
       }
     }
-  }
-  if (!is_v) {
+    uint32_t(&shared_largest)[8] = warp_largest[(head - head0) & 1];
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if ((threadIdx.x & 31) == 0) shared_largest[threadIdx.x >> 5] = largest;
+    __syncthreads();  // the buffers alternate: one barrier a head
+    largest = shared_largest[0];
+    for (unsigned w = 1; w < blockDim.x / 32; ++w) largest = max(largest, shared_largest[w]);
+    float s = fmaxf(fmaxf(__fdiv_rn(__uint_as_float(largest), 127.f), kSmallestScale), before);
+    const bool finite = largest < kInfBits && before == before;
+    if (!finite) s = __uint_as_float(0x7fc00000u);
+    if (threadIdx.x == 0 && !(s == before)) (is_v ? c.v_scales : c.k_scales)[block * c.heads + head] = s;
+
+    const bool grew = finite && first > 0 && s > before;
+    if (grew && any_old) {
+      // The older tokens' codes follow the scale: rare (a running maximum over a block's tokens).
+      const float ratio = __fdiv_rn(before, s);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (slot0 + j >= first && slot0 + j < stop)
-        *reinterpret_cast<uint2*>(codes + (slot0 + j) * c.dim + part * 8) = make_uint2(word[2 * j], word[2 * j + 1]);
-  } else if (slot0 >= first && slot0 + 4 <= stop) {
+      for (int j = 0; j < 4; ++j) {
+        if (slot0 + j >= first) continue;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0) = word[i];
-  } else if (slot0 + 4 > first && slot0 < stop) {
-    // A word that older or later slots share: only the new slots' bytes are touched.
+        for (int i = 0; i < 8; ++i) {
+          uint32_t& w = word[is_v ? i : 2 * j + i / 4];
+          const int at = is_v ? j : i & 3;
+          w = with_code(w, at, rescaled(code_value(w, at), before, s, ratio));
+        }
+      }
+    }
+    if (any_new) {
+      const float inv = __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+      for (int j = 0; j < 4; ++j) {
+        if (!is_new(j)) continue;
+        float x[8], code[8];
+        here[j].values(x);
+        bool near_tie = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = quotient(x[i], s, inv, near_tie);
+        if (near_tie) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) code[i] = quotient_at_tie(x[i], s, code[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t& w = word[is_v ? i : 2 * j + i / 4];
+          w = with_code(w, is_v ? j : i & 3, finite ? code[i] : kWhole);
+        }
+      }
+    }
+    if (is_v) {
+      if (any_new || (grew && any_old)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0) = word[i];
+      }
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (slot0 + j >= first && slot0 + j < stop)
-          codes[(part * 8 + i) * c.tokens + slot0 + j] = static_cast<int8_t>(code_at(word[i], j));
+        if (is_new(j) || (grew && slot0 + j < first))
+          *reinterpret_cast<uint2*>(codes + (slot0 + j) * c.dim + part * 8) = make_uint2(word[2 * j], word[2 * j + 1]);
+    }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
+  if (blockIdx.z)
+    append_block<T, true>(p);
+  else
+    append_block<T, false>(p);
 }
 
 struct ReadParams {
@@ -189,19 +268,19 @@ struct ReadParams {
   const int32_t *starts, *lengths, *offsets;
   int64_t rows;
   int32_t batch;
+  int32_t heads_each;
   int32_t* status;
 };
 
-// The same division of a block among threads as in the write, the other way round.
-template <typename T>
-__global__ void kv_read_kernel(const ReadParams p) {
+// The same division of a block among threads, and of heads among CTAs, as in the write, the other way round.
+template <typename T, bool is_v>
+__device__ __forceinline__ void read_block(const ReadParams& p) {
   const Cache& c = p.cache;
-  const bool is_v = blockIdx.z;
-  const int head = blockIdx.y;
   const int parts = c.dim / 8, groups = c.tokens / 4;
   const int part = is_v ? threadIdx.x / groups : threadIdx.x % parts;
   const int slot0 = 4 * (is_v ? threadIdx.x % groups : threadIdx.x / parts);
-  T* out = static_cast<T*>(is_v ? p.v_out : p.k_out) + static_cast<int64_t>(head) * c.dim + part * 8;
+  const int head0 = blockIdx.y * p.heads_each, head_end = min(head0 + p.heads_each, c.heads);
+  T* out = static_cast<T*>(is_v ? p.v_out : p.k_out) + part * 8;
   const int64_t step = static_cast<int64_t>(c.heads) * c.dim;
   const Piece piece = find_piece(p.batch, blockIdx.x, [&](int32_t b) {
     const int64_t n = rows_of(p.offsets, b, p.rows, p.status).count, start = max(p.starts[b], 0);
@@ -213,7 +292,8 @@ __global__ void kv_read_kernel(const ReadParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t r = (piece.index << c.token_bits) + slot0 + j;
-      if (r < rest.count) store8(out + (rest.begin + r) * step, none);
+      if (r < rest.count)
+        for (int head = head0; head < head_end; ++head) store8(out + (rest.begin + r) * step + head * c.dim, none);
     }
     return;
   }
@@ -223,43 +303,66 @@ __global__ void kv_read_kernel(const ReadParams p) {
   const int first = static_cast<int>(max(from, start) - start);
   const int stop = static_cast<int>(min(from + rows.count, start + c.tokens) - start);
   const int held = static_cast<int>(min(max(p.lengths[piece.sequence] - start, int64_t{0}), int64_t{stop}));
-  const int64_t row = rows.begin + start - from;  // of slot 0
-  float s = 0.f;
-  uint32_t word[8];
+  out += (rows.begin + start - from) * step;
+  int64_t block = -1;
+  if (held > first) block = block_of(c, p.table, piece.sequence, page, p.status);
+  const bool any = slot0 + 4 > first && slot0 < held && block >= 0;
+
+  uint32_t next[8];
+  float next_scale = held > first ? __uint_as_float(0x7fc00000u) : 0.f;  // (a bad block)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) word[i] = 0;
-  if (held > first) {
-    const int64_t block = block_of(c, p.table, piece.sequence, page, p.status);
-    if (block < 0) {
-      s = __uint_as_float(0x7fc00000u);
+  for (int i = 0; i < 8; ++i) next[i] = 0;
+  auto fetch = [&](int head) {
+    if (!any) return;
+    next_scale = (is_v ? c.v_scales : c.k_scales)[block * c.heads + head];
+    const int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
+    if (is_v) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        next[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0));
     } else {
-      s = (is_v ? c.v_scales : c.k_scales)[block * c.heads + head];
-      const int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
-      if (is_v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          word[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8));
-          word[2 * j] = w.x;
-          word[2 * j + 1] = w.y;
-        }
+      for (int j = 0; j < 4; ++j) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8));
+        next[2 * j] = w.x;
+        next[2 * j + 1] = w.y;
       }
     }
-  }
+  };
+  fetch(head0);
+  for (int head = head0; head < head_end; ++head) {
+    uint32_t word[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (slot0 + j < first || slot0 + j >= stop) continue;
-    float x[8];
+    for (int i = 0; i < 8; ++i) word[i] = next[i];
+    const float s = next_scale;
+    if (head + 1 < head_end) fetch(head + 1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int code = is_v ? code_at(word[i], j) : code_at(word[2 * j + i / 4], i & 3);
-      x[i] = slot0 + j < held ? static_cast<float>(code) * s : 0.f;
+    for (int j = 0; j < 4; ++j) {
+      if (slot0 + j < first || slot0 + j >= stop) continue;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float code = is_v ? code_value(word[i], j) : code_value(word[2 * j + i / 4], i & 3);
+        x[i] = slot0 + j < held ? code * s : 0.f;
+      }
+      store8(out + (slot0 + j) * step + head * c.dim, x);
     }
-    store8(out + (row + slot0 + j) * step, x);
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
+  if (blockIdx.z)
+    read_block<T, true>(p);
+  else
+    read_block<T, false>(p);
+}
+
+// Heads for one CTA: as many as leave twelve CTAs to an SM (a power of two, so that little is left over).
+int heads_for(int64_t pieces, int heads, int sms) {
+  int each = 1;
+  while (each < heads && pieces * 2 * ceil_div(heads, 2 * each) >= 12LL * sms) each *= 2;
+  return each;
 }
 
 bool table_ok(const int32_t* table, int64_t batch, int64_t stride, int64_t width) {
@@ -305,7 +408,8 @@ extern "C" int b200_kv_append(const b200_kv_append_desc* desc, void* stream) {
   p.status = kernel_status_word();
   // n new tokens touch at most (n - 2) / tokens + 2 blocks; one token each, one block each
   const int64_t pieces = !d.offsets && d.rows == d.batch ? d.batch : d.rows / d.cache.block_tokens + 2 * d.batch;
-  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(d.cache.heads), 2);
+  p.heads_each = heads_for(pieces, d.cache.heads, device_info().sm_count);
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(ceil_div(d.cache.heads, p.heads_each)), 2);
   const unsigned threads = static_cast<unsigned>(d.cache.block_tokens / 4 * (d.cache.dim / 8));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d.dtype == B200_F32)
@@ -343,7 +447,8 @@ extern "C" int b200_kv_read(const b200_kv_read_desc* desc, void* stream) {
   p.status = kernel_status_word();
   // two partial blocks a sequence at most, and the rows behind the last sequence
   const int64_t pieces = d.rows / d.cache.block_tokens + 2 * d.batch + 1;
-  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(d.cache.heads), 2);
+  p.heads_each = heads_for(pieces, d.cache.heads, device_info().sm_count);
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(ceil_div(d.cache.heads, p.heads_each)), 2);
   const unsigned threads = static_cast<unsigned>(d.cache.block_tokens / 4 * (d.cache.dim / 8));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d.dtype == B200_F32)

@@ -20,27 +20,43 @@ struct Piece {
 };
 
 // The `target`-th piece when sequence b consists of count(b) >= 0 pieces, one sequence after the
-// other. All 32 lanes call it together and get the same answer.
+// other. All 32 lanes call it together and get the same answer. Each lane first sums a 32nd of the
+// sequences (independent loads: one memory latency, whatever the batch), then the lanes go through the
+// 32nd that the piece lies in.
 template <class Count>
 __device__ __forceinline__ Piece find_piece(int32_t batch, int64_t target, const Count& count) {
   const int lane = threadIdx.x & 31;
-  int64_t before = 0;
-  for (int32_t base = 0; base < batch; base += 32) {
-    const int64_t mine = base + lane < batch ? count(base + lane) : 0;
-    int64_t upto = mine;  // inclusive sum over the lanes
+  const int32_t share = (batch + 31) / 32;
+  auto upto_lane = [&](int64_t mine) {  // inclusive sum over the lanes
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
+      const int64_t other = __shfl_up_sync(0xffffffffu, mine, o);
+      if (lane >= o) mine += other;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, before + upto > target);
-    if (past) {
-      const int first = __ffs(past) - 1;
-      return Piece{base + first, target - before - __shfl_sync(0xffffffffu, upto - mine, first)};
+    return mine;
+  };
+  int64_t mine = 0;
+#pragma unroll 4
+  for (int32_t i = 0; i < share; ++i)
+    if (lane * share + i < batch) mine += count(lane * share + i);
+  int64_t upto = upto_lane(mine);
+  const unsigned past = __ballot_sync(0xffffffffu, upto > target);
+  if (!past) return Piece{-1, target - __shfl_sync(0xffffffffu, upto, 31)};
+  int32_t first = __ffs(past) - 1;
+  int64_t before = __shfl_sync(0xffffffffu, upto - mine, first);
+  first *= share;
+  for (int32_t base = first; share > 1; base += 32) {
+    mine = base + lane < min(first + share, batch) ? count(base + lane) : 0;
+    upto = before + upto_lane(mine);
+    const unsigned here = __ballot_sync(0xffffffffu, upto > target);
+    if (here) {
+      first = base + __ffs(here) - 1;
+      before = __shfl_sync(0xffffffffu, upto - mine, __ffs(here) - 1);
+      break;
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    before = __shfl_sync(0xffffffffu, upto, 31);
   }
-  return Piece{-1, target - before};
+  return Piece{first, target - before};
 }
 
 // Rows [begin, begin + count) of sequence b in a packed tensor of `total` rows. Offsets that

@@ -22,7 +22,6 @@ from ctypes import c_int64
 from ctypes import c_size_t
 from ctypes import c_uint64
 from ctypes import c_void_p
-import math
 import os
 from pathlib import Path
 import struct
@@ -416,8 +415,6 @@ def stream_ptr(device: torch.device) -> int:
     return _raw_stream(index)
 
 
-_POOLED_BYTES = 4 * 1024 * 1024  # output_pool.MIN_BYTES, which imports this module
-
 _NO_SWITCH = contextlib.nullcontext()
 
 
@@ -448,15 +445,6 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
 def raw_stream(index: int) -> int:
     """:func:`stream_ptr` of a device by its index."""
     return _raw_stream(index)
-
-
-def new_output(shape: tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """An uninitialised result: large ones from the output pool, small ones (which it never takes) without asking it."""
-    if math.prod(shape) * dtype.itemsize < _POOLED_BYTES:
-        return torch.empty(shape, dtype=dtype, device=device)
-    from . import output_pool
-
-    return output_pool.empty(tuple(shape), dtype=dtype, device=device)
 
 
 def index_of(*tensors: torch.Tensor | None) -> int:

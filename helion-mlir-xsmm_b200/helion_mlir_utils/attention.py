@@ -159,7 +159,7 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
         else:
             q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
         rows, heads, dim = q.shape
-        out = native.new_output(q.shape, q.dtype, q.device)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         result = native.module().b200_attention_packed(
             _PACK_PACKED(code, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *q.stride()[:2],
                          *k.stride()[:2], *v.stride()[:2], rows, k.shape[0], offsets.shape[0] - 1, heads, k.shape[1], dim,

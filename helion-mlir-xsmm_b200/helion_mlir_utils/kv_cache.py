@@ -162,7 +162,7 @@ def cache_read(cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor
     offsets_ptr = _indices("cache_read", "offsets", offsets, batch + 1)
     index = native.index_of(*cache, block_table, starts, lengths, offsets)
     with native.on_index(index):
-        k, v = native.new_output((2, rows, heads, dim), dtype, block_table.device).unbind(0)
+        k, v = torch.empty((2, rows, heads, dim), dtype=dtype, device=block_table.device).unbind(0)
         result = native.module().b200_kv_read(
             _PACK_READ(*fields, code, 0, k.data_ptr(), v.data_ptr(), block_table.data_ptr(), starts_ptr, lengths_ptr, offsets_ptr,
                        stride, width, batch, rows),
@@ -200,7 +200,7 @@ def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], bl
     with native.on_index(index):
         if q.stride(-1) != 1:
             q = q.contiguous()
-        out = native.new_output(q.shape, q.dtype, q.device)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
         def desc(workspace: int, held: int) -> bytes:
             return _PACK_CACHED(*fields, code, 1.0 / math.sqrt(dim) if scale is None else scale, q.data_ptr(), out.data_ptr(),
