@@ -107,15 +107,14 @@ struct AppendParams {
   const int32_t *lengths, *offsets;      // lengths before; offsets NULL: `each` new tokens per sequence
   int64_t rows;
   int32_t batch, each;
-  int32_t heads_each;  // heads that one CTA takes, one after the other
   int32_t* status;
 };
 
 // A thread holds 8 values of each of 4 consecutive tokens. Threads of a warp go along the head first
 // for K (8 code bytes of a token next to each other) and along the tokens first for V (4 codes of a
-// channel in one word, the words of a channel next to each other), so both leave in whole sectors. Where there is
-// work for all SMs a CTA goes over several heads, with the next head's values on their way while it reduces and
-// stores: finding its block (four dependent loads) is done once, and memory is not idle in between.
+// channel in one word, the words of a channel next to each other), so both leave in whole sectors. A CTA is one chain of
+// dependent loads (lengths, then its values and the table, then the block's scale and codes): what counts is how many
+// are on an SM, so registers are held to four CTAs of 256 threads.
 template <typename T, bool is_v>
 __device__ __forceinline__ void append_block(const AppendParams& p) {
   const Cache& c = p.cache;
@@ -133,128 +132,116 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
   const Rows rows = new_rows(piece.sequence);
   const int64_t length = max(p.lengths[piece.sequence], 0);
   const int64_t page = (length >> c.token_bits) + piece.index;
-  const int64_t block = block_of(c, p.table, piece.sequence, page, p.status);
-  if (block < 0) return;
   const int64_t start = page << c.token_bits;
   const int first = static_cast<int>(max(length, start) - start);  // slots [first, stop) are new
   const int stop = static_cast<int>(min(length + rows.count, start + c.tokens) - start);
 
-  const int parts = c.dim / 8, groups = c.tokens / 4;
+  const int head = blockIdx.y, parts = c.dim / 8, groups = c.tokens / 4;
   const int part = is_v ? threadIdx.x / groups : threadIdx.x % parts;
   const int slot0 = 4 * (is_v ? threadIdx.x % groups : threadIdx.x / parts);
-  const int64_t step = is_v ? p.v_row : p.k_row, head_step = is_v ? p.v_head : p.k_head;
-  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + part * 8 + (rows.begin + start - length) * step;
+  const int64_t step = is_v ? p.v_row : p.k_row;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + part * 8 + (rows.begin + start - length) * step +
+                 head * (is_v ? p.v_head : p.k_head);
   auto is_new = [&](int j) { return slot0 + j >= first && slot0 + j < stop; };
   const bool any_new = slot0 + 4 > first && slot0 < stop, all_new = slot0 >= first && slot0 + 4 <= stop;
   const bool any_old = slot0 < first;
 
-  __shared__ uint32_t warp_largest[2][8];
-  const int head0 = blockIdx.y * p.heads_each, head_end = min(head0 + p.heads_each, c.heads);
-  Eight<T> next[4];
-  float next_scale = 0.f;
-  auto fetch = [&](int head) {
+  Eight<T> here[4];  // on their way while the block is looked up
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (is_new(j))
-        next[j].load(src + head * head_step + (slot0 + j) * step);
-      else
-        next[j].clear();
-    }
-    if (first > 0) next_scale = (is_v ? c.v_scales : c.k_scales)[block * c.heads + head];
-  };
-  fetch(head0);
-  for (int head = head0; head < head_end; ++head) {
-    Eight<T> here[4];
-    uint32_t largest = 0;
+  for (int j = 0; j < 4; ++j) {
+    if (is_new(j))
+      here[j].load(src + (slot0 + j) * step);
+    else
+      here[j].clear();
+  }
+  const int64_t block = block_of(c, p.table, piece.sequence, page, p.status);
+  if (block < 0) return;
+  float* scale = (is_v ? c.v_scales : c.k_scales) + block * c.heads + head;
+  const float before = first > 0 ? *scale : 0.f;
+  int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
+  // K: two words of each token; V: one word of each channel. What is there counts only where older
+  // tokens or bytes of other slots share a word.
+  uint32_t word[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      here[j] = next[j];
-      largest = max(largest, here[j].largest());
-    }
-    const float before = next_scale;
-    if (head + 1 < head_end) fetch(head + 1);
-    int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
-    // K: two words of each token; V: one word of each channel. What is there counts only where older
-    // tokens or bytes of other slots share a word.
-    uint32_t word[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) word[i] = 0;
-    if (is_v ? (any_old || any_new) && !all_new : any_old) {
-      if (is_v) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) word[i] = *reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint2 w = *reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8);
-          word[2 * j] = w.x;
-          word[2 * j + 1] = w.y;
-        }
-      }
-    }
-    uint32_t(&shared_largest)[8] = warp_largest[(head - head0) & 1];
-    largest = __reduce_max_sync(0xffffffffu, largest);
-    if ((threadIdx.x & 31) == 0) shared_largest[threadIdx.x >> 5] = largest;
-    __syncthreads();  // the buffers alternate: one barrier a head
-    largest = shared_largest[0];
-    for (unsigned w = 1; w < blockDim.x / 32; ++w) largest = max(largest, shared_largest[w]);
-    float s = fmaxf(fmaxf(__fdiv_rn(__uint_as_float(largest), 127.f), kSmallestScale), before);
-    const bool finite = largest < kInfBits && before == before;
-    if (!finite) s = __uint_as_float(0x7fc00000u);
-    if (threadIdx.x == 0 && !(s == before)) (is_v ? c.v_scales : c.k_scales)[block * c.heads + head] = s;
-
-    const bool grew = finite && first > 0 && s > before;
-    if (grew && any_old) {
-      // The older tokens' codes follow the scale: rare (a running maximum over a block's tokens).
-      const float ratio = __fdiv_rn(before, s);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (slot0 + j >= first) continue;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t& w = word[is_v ? i : 2 * j + i / 4];
-          const int at = is_v ? j : i & 3;
-          w = with_code(w, at, rescaled(code_value(w, at), before, s, ratio));
-        }
-      }
-    }
-    if (any_new) {
-      const float inv = __frcp_rn(s);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!is_new(j)) continue;
-        float x[8], code[8];
-        here[j].values(x);
-        bool near_tie = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) code[i] = quotient(x[i], s, inv, near_tie);
-        if (near_tie) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) code[i] = quotient_at_tie(x[i], s, code[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t& w = word[is_v ? i : 2 * j + i / 4];
-          w = with_code(w, is_v ? j : i & 3, finite ? code[i] : kWhole);
-        }
-      }
-    }
+  for (int i = 0; i < 8; ++i) word[i] = 0;
+  if (is_v ? (any_old || any_new) && !all_new : any_old) {
     if (is_v) {
-      if (any_new || (grew && any_old)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0) = word[i];
-      }
+      for (int i = 0; i < 8; ++i) word[i] = *reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (is_new(j) || (grew && slot0 + j < first))
-          *reinterpret_cast<uint2*>(codes + (slot0 + j) * c.dim + part * 8) = make_uint2(word[2 * j], word[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) {
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8);
+        word[2 * j] = w.x;
+        word[2 * j + 1] = w.y;
+      }
     }
+  }
+  __shared__ uint32_t warp_largest[8];
+  uint32_t largest = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) largest = max(largest, here[j].largest());
+  largest = __reduce_max_sync(0xffffffffu, largest);
+  if ((threadIdx.x & 31) == 0) warp_largest[threadIdx.x >> 5] = largest;
+  __syncthreads();
+  largest = warp_largest[0];
+  for (unsigned w = 1; w < blockDim.x / 32; ++w) largest = max(largest, warp_largest[w]);
+  float s = fmaxf(fmaxf(__fdiv_rn(__uint_as_float(largest), 127.f), kSmallestScale), before);
+  const bool finite = largest < kInfBits && before == before;
+  if (!finite) s = __uint_as_float(0x7fc00000u);
+  if (threadIdx.x == 0 && !(s == before)) *scale = s;  // (every thread has read it before the barrier)
+
+  const bool grew = finite && first > 0 && s > before;
+  if (grew && any_old) {
+    // The older tokens' codes follow the scale: rare (a running maximum over a block's tokens).
+    const float ratio = __fdiv_rn(before, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (slot0 + j >= first) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t& w = word[is_v ? i : 2 * j + i / 4];
+        const int at = is_v ? j : i & 3;
+        w = with_code(w, at, rescaled(code_value(w, at), before, s, ratio));
+      }
+    }
+  }
+  if (any_new) {
+    const float inv = __frcp_rn(s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!is_new(j)) continue;
+      float x[8], code[8];
+      here[j].values(x);
+      bool near_tie = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) code[i] = quotient(x[i], s, inv, near_tie);
+      if (near_tie) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = quotient_at_tie(x[i], s, code[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t& w = word[is_v ? i : 2 * j + i / 4];
+        w = with_code(w, is_v ? j : i & 3, finite ? code[i] : kWhole);
+      }
+    }
+  }
+  if (is_v) {
+    if (any_new || (grew && any_old)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0) = word[i];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (is_new(j) || (grew && slot0 + j < first))
+        *reinterpret_cast<uint2*>(codes + (slot0 + j) * c.dim + part * 8) = make_uint2(word[2 * j], word[2 * j + 1]);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) kv_append_kernel(const AppendParams p) {
   if (blockIdx.z)
     append_block<T, true>(p);
   else
@@ -272,7 +259,7 @@ struct ReadParams {
   int32_t* status;
 };
 
-// The same division of a block among threads, and of heads among CTAs, as in the write, the other way round.
+// The same division of a block among threads as in the write, the other way round.
 template <typename T, bool is_v>
 __device__ __forceinline__ void read_block(const ReadParams& p) {
   const Cache& c = p.cache;
@@ -408,8 +395,7 @@ extern "C" int b200_kv_append(const b200_kv_append_desc* desc, void* stream) {
   p.status = kernel_status_word();
   // n new tokens touch at most (n - 2) / tokens + 2 blocks; one token each, one block each
   const int64_t pieces = !d.offsets && d.rows == d.batch ? d.batch : d.rows / d.cache.block_tokens + 2 * d.batch;
-  p.heads_each = heads_for(pieces, d.cache.heads, device_info().sm_count);
-  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(ceil_div(d.cache.heads, p.heads_each)), 2);
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(d.cache.heads), 2);
   const unsigned threads = static_cast<unsigned>(d.cache.block_tokens / 4 * (d.cache.dim / 8));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d.dtype == B200_F32)
