@@ -53,6 +53,7 @@ struct CachedParams {
   int32_t batch, tokens, heads, group;
   int32_t rows, row_tiles;  // query rows of a (sequence, key/value head): tokens * group, row = token * group + head within the group
   int32_t workers;
+  int32_t q_vectors;  // q can be read as 16-byte vectors
   float scale_log2;
   float* partial;  // [workers][2][rows of a tile x (2 + dim)]
   int32_t* status;
@@ -64,23 +65,32 @@ __device__ __forceinline__ int64_t capacity_of(const CachedParams& p) {
   return static_cast<int64_t>(p.table.width) << p.cache.token_bits;
 }
 // Tiles of one (sequence, head, row tile). A sequence that its table cannot hold has none: it is answered with NaN.
-__device__ __forceinline__ int64_t tiles_of(const CachedParams& p, int32_t b) {
+__device__ __forceinline__ int32_t tiles_of(const CachedParams& p, int32_t b) {
   const int64_t length = p.lengths[b];
-  return length <= 0 || length > capacity_of(p) ? 0 : (length + kTileTokens - 1) / kTileTokens;
+  return length <= 0 || length > capacity_of(p) ? 0 : static_cast<int32_t>((length + kTileTokens - 1) / kTileTokens);
 }
-__device__ __forceinline__ int64_t total_tiles(const CachedParams& p) {
-  int64_t sum = 0;
-  for (int32_t b = threadIdx.x & 31; b < p.batch; b += 32) sum += tiles_of(p, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * p.cache.heads * p.row_tiles;
+// Tiles of all sequences (the launch made sure that 32 bits hold them), and of those before sequence `upto`.
+__device__ __forceinline__ int32_t count_tiles(const CachedParams& p, int32_t upto, int32_t& before) {
+  int32_t sum = 0;
+  before = 0;
+#pragma unroll 4
+  for (int32_t b = threadIdx.x & 31; b < p.batch; b += 32) {
+    const int32_t tiles = tiles_of(p, b);
+    sum += tiles;
+    if (b < upto) before += tiles;
+  }
+  const int32_t pairs = p.cache.heads * p.row_tiles;
+  before = __reduce_add_sync(0xffffffffu, before) * pairs;
+  return __reduce_add_sync(0xffffffffu, sum) * pairs;
 }
-__device__ __forceinline__ int64_t tiles_per_worker(const CachedParams& p, int64_t total) {
+__device__ __forceinline__ int32_t tiles_per_worker(const CachedParams& p, int32_t total) {
   return (total + p.workers - 1) / p.workers;
 }
+// What a worker leaves of a pair that it did not do alone: maximum and sum of each row, then the accumulator. In slot 1 if
+// the pair began with this worker, in slot 0 otherwise (a worker has one of either at most).
 template <int ROWS, int D>
-__device__ __forceinline__ float* partial_of(const CachedParams& p, int64_t worker, int slot) {
-  return p.partial + (worker * 2 + slot) * (ROWS * (2 + D));
+__device__ __forceinline__ float* partial_of(const CachedParams& p, int32_t worker, int slot) {
+  return p.partial + static_cast<int64_t>(worker * 2 + slot) * (ROWS * (2 + D));
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -129,8 +139,7 @@ __device__ __forceinline__ void word_loads_arrive(uint32_t bar) {
 
 // Where a worker stands in the line of tiles.
 struct Cursor {
-  int32_t b, h, rt;
-  int64_t tile, tiles;
+  int32_t b, h, rt, tile, tiles;
 };
 __device__ __forceinline__ void advance(const CachedParams& p, Cursor& c) {
   if (++c.tile < c.tiles) return;
@@ -174,23 +183,25 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
   }
   if (threadIdx.x == 0) *abort_flag = 0;
   __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;");  // the joining kernel may come up (it waits for this one's end)
 
   const Cache& c = p.cache;
-  const int64_t total = total_tiles(p), each = tiles_per_worker(p, total);
+  int32_t none_before;
+  const int32_t total = count_tiles(p, 0, none_before), each = tiles_per_worker(p, total);
   // neighbouring workers on different SMs: little work spreads over all of them
-  const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
-  const int64_t begin = worker * each, end = min(begin + each, total);
-  if (worker >= p.workers || begin >= end) return;
+  const int32_t worker = warp * gridDim.x + blockIdx.x;
+  if (worker >= p.workers || static_cast<int64_t>(worker) * each >= total) return;
+  const int32_t begin = worker * each, end = static_cast<int32_t>(min(static_cast<int64_t>(begin) + each, static_cast<int64_t>(total)));
 
   Cursor at;
   {
-    const Piece piece = find_piece(p.batch, begin, [&](int32_t b) { return tiles_of(p, b) * c.heads * p.row_tiles; });
+    const Piece piece = find_piece(p.batch, begin, [&](int32_t b) { return int64_t{tiles_of(p, b)} * c.heads * p.row_tiles; });
     at.b = piece.sequence;
     at.tiles = tiles_of(p, at.b);
-    const int64_t pair = piece.index / at.tiles;
-    at.tile = piece.index - pair * at.tiles;
-    at.h = static_cast<int32_t>(pair / p.row_tiles);
-    at.rt = static_cast<int32_t>(pair - static_cast<int64_t>(at.h) * p.row_tiles);
+    const int32_t index = static_cast<int32_t>(piece.index), pair = index / at.tiles;
+    at.tile = index - pair * at.tiles;
+    at.h = pair / p.row_tiles;
+    at.rt = pair - at.h * p.row_tiles;
   }
 
   // -------------------------------------------------------------------- copies
@@ -199,14 +210,14 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
   const int pages_full = kTileTokens >> c.token_bits;
   const uint32_t page_bytes = static_cast<uint32_t>(D) << c.token_bits;
   const uint32_t v_page_step = page_bytes + (c.token_bits == 4 ? 32u : 64u);
-  const int64_t units = end - begin, items = 2 * units;
+  const int32_t items = 2 * (end - begin);
   Cursor ahead = at;
-  int64_t next_item = 0;
+  int32_t next_item = 0;
   uint32_t next_slot = 0;
   int32_t next_block = -1;
   bool next_held = false;  // whether a position of this lane's page exists
   auto look_up = [&]() {   // the block of this lane's page of the next unit
-    const int64_t page = ahead.tile * pages_full + lane;
+    const int64_t page = static_cast<int64_t>(ahead.tile) * pages_full + lane;
     const int64_t held = (static_cast<int64_t>(p.lengths[ahead.b]) + c.tokens - 1) >> c.token_bits;
     next_held = lane < pages_full && page < held;
     next_block = next_held ? p.table.blocks[ahead.b * p.table.stride + page] : -1;
@@ -257,10 +268,10 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
   uint32_t q_hi[kSteps][NT][2], q_lo[kSplit ? kSteps : 1][kSplit ? NT : 1][2];
   float o[kSteps][NT][4], row_scale[NT][2], top[NT][2], sum[NT][2];
   int64_t limit[NT][2];  // positions that the row sees
-  int64_t segment = begin - at.tile;
+  int32_t segment = begin - at.tile;  // where the pair in work began
   bool fresh = true;
 
-  for (int64_t unit = begin; unit < end; ++unit) {
+  for (int32_t unit = begin; unit < end; ++unit) {
     if (fresh) {
       // Queries of this (sequence, head): row `octet` of each row tile, the 16 consecutive dims per 64 that
       // belong to this quad; scaled by a power of two that brings the row's largest to [1, 2).
@@ -273,11 +284,21 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
         const bool real = row < p.rows;
         const int token = row / p.group, head = at.h * p.group + row % p.group;
         const T* src = static_cast<const T*>(p.q) + at.b * p.q_batch + token * p.q_token + head * p.q_head;
+        constexpr int kVec = Elem<T>::kVec;
+        if (real && p.q_vectors) {
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i) {
-          x[i] = real ? Elem<T>::load(src + (i / 16) * 64 + quad * 16 + i % 16) : 0.f;
-          largest = max(largest, __float_as_uint(x[i]) & 0x7fffffffu);
+          for (int i = 0; i < D / 4; i += kVec) {
+            float part[kVec];
+            unpack16(ld_plain16(src + (i / 16) * 64 + quad * 16 + i % 16), part);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) x[i + e] = part[e];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i) x[i] = real ? Elem<T>::load(src + (i / 16) * 64 + quad * 16 + i % 16) : 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) largest = max(largest, __float_as_uint(x[i]) & 0x7fffffffu);
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const uint32_t power = min(max(largest & 0x7f800000u, 27u << 23), 253u << 23);
@@ -348,8 +369,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
 
     // Softmax: this thread has 8 tokens of two rows for each row tile.
     const float v_log = log2f(v_scale);
-    const int64_t first_token = at.tile * kTileTokens + 16 * (octet >> 1) + (octet & 1);
-    const bool cut = at.tile * kTileTokens + kTileTokens > p.lengths[at.b] - p.tokens + 1;
+    const int64_t first_token = static_cast<int64_t>(at.tile) * kTileTokens + 16 * (octet >> 1) + (octet & 1);
+    const bool cut = (at.tile + int64_t{1}) * kTileTokens > static_cast<int64_t>(p.lengths[at.b]) - p.tokens + 1;
     uint32_t p_hi[4][NT][2], p_lo[kSplit ? 4 : 1][kSplit ? NT : 1][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -474,77 +495,91 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
   }
 }
 
-// Joins what several workers left of one row: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w. One CTA per
-// (sequence, head, row tile) and row; its warps take the workers in turn, and their sums are added in the order of the warps.
-template <typename T, int D, int NT>
+// Joins what several workers left of a row: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w, the workers in order. A CTA's
+// eight warps take eight rows of one (sequence, head, row tile), or, where there are few of those (SPLIT 8), one row: each an
+// eighth of the workers, added in order. It comes up while the first kernel runs and waits for its end before it reads.
+template <typename T, int D, int NT, int SPLIT>
 __global__ void __launch_bounds__(256) cached_join_kernel(const CachedParams p) {
-  constexpr int kRows = 8 * NT, kPer = D / 32;
-  __shared__ float best_of[8], sum_of[8], acc_of[8][D];
+  constexpr int kRows = 8 * NT, kPer = D / 32, kStride = kRows * (2 + D);
+  __shared__ float best_of[8], sum_of[8], acc_of[SPLIT > 1 ? 8 : 1][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t pairs = static_cast<int64_t>(p.cache.heads) * p.row_tiles;
-  const int32_t b = static_cast<int32_t>(blockIdx.x / pairs);
-  const int64_t pair = blockIdx.x - b * pairs;
-  const int32_t h = static_cast<int32_t>(pair / p.row_tiles), rt = static_cast<int32_t>(pair - h * static_cast<int64_t>(p.row_tiles));
-  const int in_tile = blockIdx.y, row = rt * kRows + in_tile;
-  if (row >= p.rows) return;
+  const int split = SPLIT > 1 ? warp : 0, in_tile = SPLIT > 1 ? blockIdx.y : blockIdx.y * 8 + warp;
+  const int32_t pairs = p.cache.heads * p.row_tiles;
+  const int32_t b = blockIdx.x / pairs, pair = blockIdx.x - b * pairs;
+  const int32_t h = pair / p.row_tiles, rt = pair - h * p.row_tiles;
+  const int row = rt * kRows + in_tile;
   const int token = row / p.group;
   const int64_t length = p.lengths[b], limit = length - p.tokens + 1 + token;
+  const int32_t tiles = tiles_of(p, b);
+  int32_t before, first = 0, last = 0;
+  const int32_t total = count_tiles(p, b, before);
+  if (tiles > 0) {
+    const int32_t each = tiles_per_worker(p, total), start = before + pair * tiles;
+    first = start / each;
+    last = (start + tiles - 1) / each;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (row >= p.rows || (tiles > 0 && first == last)) return;  // no such row, or finished by its worker (CTA-wide if SPLIT)
   T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(b) * p.tokens + token) * p.heads + h * p.group + row % p.group) * D;
-  const int64_t tiles = tiles_of(p, b);
   if (tiles == 0) {
     const bool beyond = length > 0;
-    if (beyond && threadIdx.x == 0 && p.status) atomicOr(p.status, kErrBlocks);
-    if (threadIdx.x < D) Elem<T>::store(dst + threadIdx.x, beyond ? __uint_as_float(0x7fc00000u) : 0.f);
+    if (beyond && lane == 0 && p.status) atomicOr(p.status, kErrBlocks);
+    if (split == 0)
+      for (int i = lane; i < D; i += 32) Elem<T>::store(dst + i, beyond ? __uint_as_float(0x7fc00000u) : 0.f);
     return;
   }
-  int64_t before = 0, all = 0;
-  for (int32_t i = lane; i < p.batch; i += 32) {
-    const int64_t t = tiles_of(p, i);
-    all += t;
-    if (i < b) before += t;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  const int64_t each = tiles_per_worker(p, all * pairs), start = before * pairs + pair * tiles;
-  const int64_t first = start / each, last = (start + tiles - 1) / each;
-  if (first == last) return;  // finished by its worker
-  auto left_by = [&](int64_t w) { return partial_of<kRows, D>(p, w, start >= w * each ? 1 : 0); };
-
+  const float* left = partial_of<kRows, D>(p, first, 1) + in_tile;  // of the first worker; the others' in slot 0
+  auto left_by = [&](int32_t w) { return left + static_cast<int64_t>((w - first) * 2 - (w > first)) * kStride; };
+  const int32_t count = last - first + 1;
+  const int32_t from = count * split / SPLIT, to = count * (split + 1) / SPLIT;  // this warp's
   float best = -INFINITY;
-  for (int64_t w = first + threadIdx.x; w <= last; w += 256) best = fmaxf(best, left_by(w)[in_tile]);
+  for (int32_t i = from + lane; i < to; i += 32) best = fmaxf(best, *left_by(first + i));
   best = warp_fmax(best);
-  if (lane == 0) best_of[warp] = best;
-  __syncthreads();
+  if (SPLIT > 1) {
+    if (lane == 0) best_of[warp] = best;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) best = fmaxf(best, best_of[i]);
+    for (int i = 0; i < 8; ++i) best = fmaxf(best, best_of[i]);
+  }
   if (best == -INFINITY) best = 0.f;
   float sum = 0.f, acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int64_t w = first + warp; w <= last; w += 8) {
-    const float* left = left_by(w);
-    const float weight = fast_exp2(left[in_tile] - best);
-    sum = fmaf(left[kRows + in_tile], weight, sum);
-    const float* x = left + 2 * kRows + in_tile * D + lane * kPer;
+  for (int32_t base = from; base < to; base += 32) {
+    float weight = 0.f;
+    if (base + lane < to) {
+      const float* mine = left_by(first + base + lane);
+      weight = fast_exp2(mine[0] - best);
+      sum = fmaf(mine[kRows], weight, sum);
+    }
+    const int here = min(32, to - base);
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
+      const float w = __shfl_sync(0xffffffffu, weight, i);
+      const float* x = left_by(first + base + i) - in_tile + 2 * kRows + in_tile * D + lane * kPer;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(x[i], weight, acc[i]);
+      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(x[e], w, acc[e]);
+    }
   }
-  if (lane == 0) sum_of[warp] = sum;
+  sum = warp_sum(sum);
+  if (SPLIT > 1) {
+    if (lane == 0) sum_of[warp] = sum;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) acc_of[warp][lane * kPer + i] = acc[i];
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  float total = 0.f, value = 0.f;
+    for (int i = 0; i < kPer; ++i) acc_of[warp][lane * kPer + i] = acc[i];
+    __syncthreads();
+    if (warp > 0) return;
+    sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    total += sum_of[i];
-    value += acc_of[i][threadIdx.x];
+    for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      sum += sum_of[w];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] += acc_of[w][lane * kPer + i];
+    }
   }
-  Elem<T>::store(dst + threadIdx.x, limit <= 0 ? 0.f : value / total);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) Elem<T>::store(dst + lane * kPer + i, limit <= 0 ? 0.f : acc[i] / sum);
 }
 
 // Query rows of a tile: 8, or 16 where a (sequence, head) has more than 8 (32 would not leave room in
@@ -552,7 +587,7 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CachedParams p) 
 int row_tile(int64_t rows) { return rows <= 8 ? 8 : 16; }
 
 struct CachedPlan {
-  int64_t rows, row_tiles, pairs, workers;
+  int64_t rows, row_tiles, pairs, most, workers;  // most: tiles, if every sequence filled its table
   int tile, grid;
 };
 CachedPlan plan_cached(const b200_cached_attention_desc& d, int sms) {
@@ -562,7 +597,7 @@ CachedPlan plan_cached(const b200_cached_attention_desc& d, int sms) {
   plan.row_tiles = ceil_div(plan.rows, plan.tile);
   plan.pairs = d.batch * d.cache.heads * plan.row_tiles;
   // no more workers than the longest possible sequences have tiles
-  const int64_t most = plan.pairs * (ceil_div(d.table_width * d.cache.block_tokens, kTileTokens) + 1);
+  const int64_t most = plan.most = plan.pairs * (ceil_div(d.table_width * d.cache.block_tokens, kTileTokens) + 1);
   plan.grid = static_cast<int>(most < sms ? most : sms);
   plan.workers = most < static_cast<int64_t>(plan.grid) * kWarps ? most : static_cast<int64_t>(plan.grid) * kWarps;
   return plan;
@@ -570,13 +605,30 @@ CachedPlan plan_cached(const b200_cached_attention_desc& d, int sms) {
 
 std::once_flag g_cached_attr_once[64];
 
+// The joining kernel as a programmatic dependent of the first: launched and set up while that one runs.
+template <typename T, int D, int NT, int SPLIT>
+cudaError_t launch_join(const CachedParams& p, const CachedPlan& plan, cudaStream_t s) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(plan.pairs), SPLIT > 1 ? 8 * NT : NT);
+  config.blockDim = dim3(256);
+  config.stream = s;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, cached_join_kernel<T, D, NT, SPLIT>, p);
+}
+
 template <typename T, int D, int NT>
-int launch_cached(const CachedParams& p, const CachedPlan& plan, cudaStream_t s) {
+int launch_cached(const CachedParams& p, const CachedPlan& plan, int sms, cudaStream_t s) {
   cached_kernel<T, D, NT><<<plan.grid, 32 * kWarps, Ring<D>::kBytes, s>>>(p);
   const int code = check_launch();
   if (code) return finish(code);
-  cached_join_kernel<T, D, NT><<<dim3(static_cast<unsigned>(plan.pairs), 8 * NT), 256, 0, s>>>(p);
-  return launched();
+  // A row has about workers / pairs partial results. With few pairs one warp would go over many of them.
+  const cudaError_t err = plan.pairs >= 2 * sms ? launch_join<T, D, NT, 1>(p, plan, s) : launch_join<T, D, NT, 8>(p, plan, s);
+  if (err != cudaSuccess) cudaGetLastError();
+  return err == cudaSuccess ? launched() : finish(-static_cast<int>(err));
 }
 template <typename T>
 void cached_attributes() {
@@ -586,9 +638,9 @@ void cached_attributes() {
   cudaFuncSetAttribute(cached_kernel<T, 128, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ring<128>::kBytes));
 }
 template <typename T>
-int launch_cached_any(const CachedParams& p, const CachedPlan& plan, int dim, cudaStream_t s) {
-  if (dim == 64) return plan.tile == 8 ? launch_cached<T, 64, 1>(p, plan, s) : launch_cached<T, 64, 2>(p, plan, s);
-  return plan.tile == 8 ? launch_cached<T, 128, 1>(p, plan, s) : launch_cached<T, 128, 2>(p, plan, s);
+int launch_cached_any(const CachedParams& p, const CachedPlan& plan, int dim, int sms, cudaStream_t s) {
+  if (dim == 64) return plan.tile == 8 ? launch_cached<T, 64, 1>(p, plan, sms, s) : launch_cached<T, 64, 2>(p, plan, sms, s);
+  return plan.tile == 8 ? launch_cached<T, 128, 1>(p, plan, sms, s) : launch_cached<T, 128, 2>(p, plan, sms, s);
 }
 
 }  // namespace
@@ -629,7 +681,7 @@ extern "C" int b200_attention_cached(const b200_cached_attention_desc* desc, voi
   const DeviceInfo& dev = device_info();
   if (dev.sm_count == 0) return refuse(B200_E_DEVICE);
   const CachedPlan plan = plan_cached(d, dev.sm_count);
-  if (plan.rows > INT32_MAX / 2 || plan.pairs > INT32_MAX) return refuse(B200_E_SHAPE);
+  if (plan.rows > INT32_MAX / 2 || plan.pairs > INT32_MAX || plan.most > INT32_MAX) return refuse(B200_E_SHAPE);
   if (!d.workspace || d.workspace_bytes < static_cast<int64_t>(workspace_for(plan, d.cache.dim)) || !aligned(d.workspace, 16))
     return refuse(B200_E_WORKSPACE);
   CachedParams p{};
@@ -648,6 +700,8 @@ extern "C" int b200_attention_cached(const b200_cached_attention_desc* desc, voi
   p.rows = static_cast<int32_t>(plan.rows);
   p.row_tiles = static_cast<int32_t>(plan.row_tiles);
   p.workers = static_cast<int32_t>(plan.workers);
+  const int64_t vec = d.dtype == B200_F32 ? 4 : 8;
+  p.q_vectors = aligned(d.q, 16) && d.q_batch % vec == 0 && d.q_token % vec == 0 && d.q_head % vec == 0;
   p.scale_log2 = d.scale * kLog2e;
   p.partial = static_cast<float*>(d.workspace);
   p.status = kernel_status_word();
@@ -656,6 +710,6 @@ extern "C" int b200_attention_cached(const b200_cached_attention_desc* desc, voi
     cached_attributes<__nv_bfloat16>();
   });
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return d.dtype == B200_F32 ? launch_cached_any<float>(p, plan, d.cache.dim, s)
-                             : launch_cached_any<__nv_bfloat16>(p, plan, d.cache.dim, s);
+  return d.dtype == B200_F32 ? launch_cached_any<float>(p, plan, d.cache.dim, dev.sm_count, s)
+                             : launch_cached_any<__nv_bfloat16>(p, plan, d.cache.dim, dev.sm_count, s);
 }
