@@ -37,7 +37,6 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileTokens = 64;
-constexpr int kWarps = 8;                 // workers of a CTA, one CTA per SM
 constexpr float kHeadroom = 10.f;         // P = 2^(t - max + 10) ...
 constexpr float kStale = 5.f;             // ... and the maximum may be 5 behind: at most 2^15 in f16
 constexpr float kSmallestScale = 7.888609052210118e-31f;
@@ -54,7 +53,7 @@ struct CachedParams {
   int32_t rows, row_tiles;  // query rows of a (sequence, key/value head): tokens * group, row = token * group + head within the group
   int32_t workers;
   int32_t q_vectors;  // q can be read as 16-byte vectors
-  float scale_log2;
+  float scale_log2, q_sign;  // |scale| * log2(e) and the scale's sign, which the queries take (a scale of 0: 1 and 0)
   float* partial;  // [workers][2][rows of a tile x (2 + dim)]
   int32_t* status;
 };
@@ -124,10 +123,18 @@ __device__ __forceinline__ void codes_to_half(uint32_t codes, uint32_t& lo, uint
   hi = *reinterpret_cast<const uint32_t*>(&b);
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(bar)
-               : "memory");
+// Codes are read once a call: they go first when L2 needs room (61 -> 57 us on 64 sequences of up to 4096: the lines
+// that stay are whole blocks that the next step finds again).
+__device__ __forceinline__ uint64_t read_once_policy() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+      : "memory");
 }
 __device__ __forceinline__ void word_load(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -156,7 +163,10 @@ __device__ __forceinline__ void advance(const CachedParams& p, Cursor& c) {
 
 template <int D>
 struct Ring {
-  static constexpr int kSlots = D == 64 ? 6 : 3;
+  static constexpr int kWarps = D == 64 ? 12 : 8;  // workers of a CTA, one CTA per SM
+  // 4 of up to 131072 positions, heads of 128, 8 warps: 107.5 us with two slots, 116 with three, 128 with four for 6 warps;
+  // 10 warps of two: 120.
+  static constexpr int kSlots = D == 64 ? 4 : 2;
   // 64 tokens of a head, plus the gap between pages that keeps V's columns on different banks
   static constexpr uint32_t kSlotBytes = kTileTokens * D + 128;
   static constexpr uint32_t kScaleBytes = 4 * 8 * 4;  // of four tiles: four pages' K and V scales
@@ -165,7 +175,7 @@ struct Ring {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedParams p) {
+__global__ void __launch_bounds__(32 * Ring<D>::kWarps, 1) cached_kernel(const CachedParams p) {
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr int kRows = 8 * NT, kSteps = D / 16, kSlots = Ring<D>::kSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -174,8 +184,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
   uint8_t* base = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
   uint8_t* ring = base + warp * Ring<D>::kWarpBytes;
   float* scales = reinterpret_cast<float*>(ring + kSlots * Ring<D>::kSlotBytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kWarps * Ring<D>::kWarpBytes) + warp * kSlots;
-  volatile int* abort_flag = reinterpret_cast<int*>(base + kWarps * (Ring<D>::kWarpBytes + kSlots * 8));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + Ring<D>::kWarps * Ring<D>::kWarpBytes) + warp * kSlots;
+  volatile int* abort_flag = reinterpret_cast<int*>(base + Ring<D>::kWarps * (Ring<D>::kWarpBytes + kSlots * 8));
   const uint32_t ring_addr = smem_u32(ring), scales_addr = smem_u32(scales), bars_addr = smem_u32(bars);
   if (lane == 0) {
     for (int s = 0; s < kSlots; ++s) mbar_init(bars_addr + 8 * s, 33);
@@ -214,31 +224,33 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
   Cursor ahead = at;
   int32_t next_item = 0;
   uint32_t next_slot = 0;
-  int32_t next_block = -1;
-  bool next_held = false;  // whether a position of this lane's page exists
+  const uint64_t policy = read_once_policy();
+  int64_t next_pair = 0;     // (block, head) of this lane's page
+  bool next_held = false;    // whether a position of it exists
+  bool next_there = false;   // and its block does
   auto look_up = [&]() {   // the block of this lane's page of the next unit
     const int64_t page = static_cast<int64_t>(ahead.tile) * pages_full + lane;
     const int64_t held = (static_cast<int64_t>(p.lengths[ahead.b]) + c.tokens - 1) >> c.token_bits;
     next_held = lane < pages_full && page < held;
-    next_block = next_held ? p.table.blocks[ahead.b * p.table.stride + page] : -1;
+    const int32_t block = next_held ? p.table.blocks[ahead.b * p.table.stride + page] : -1;
+    next_there = block >= 0 && block < c.blocks;
+    next_pair = static_cast<int64_t>(block) * c.heads + ahead.h;
   };
   auto issue = [&]() {
     const uint32_t bar = bars_addr + 8 * next_slot;
     const bool is_v = next_item & 1;
-    const bool there = next_block >= 0 && next_block < c.blocks;
-    const unsigned copies = __ballot_sync(0xffffffffu, there);
+    const unsigned copies = __ballot_sync(0xffffffffu, next_there);
     if (lane == 0) mbar_expect_tx(bar, __popc(copies) * page_bytes);
     __syncwarp();
-    const int64_t pair = static_cast<int64_t>(next_block) * c.heads + ahead.h;
-    if (there) {
+    if (next_there) {
       const uint32_t dst = ring_addr + next_slot * Ring<D>::kSlotBytes + lane * (is_v ? v_page_step : page_bytes);
-      bulk_load(dst, (is_v ? c.v_codes : c.k_codes) + pair * page_bytes, page_bytes, bar);
+      bulk_load(dst, (is_v ? c.v_codes : c.k_codes) + next_pair * page_bytes, page_bytes, bar, policy);
     }
     if (!is_v && next_held) {
       const uint32_t dst = scales_addr + (static_cast<uint32_t>(next_item >> 1) & 3u) * 32 + lane * 4;
-      word_load(dst, there ? c.k_scales + pair : &g_not_a_number);
-      word_load(dst + 16, there ? c.v_scales + pair : &g_not_a_number);
-      if (!there && p.status) atomicOr(p.status, kErrBlocks);
+      word_load(dst, next_there ? c.k_scales + next_pair : &g_not_a_number);
+      word_load(dst + 16, next_there ? c.v_scales + next_pair : &g_not_a_number);
+      if (!next_there && p.status) atomicOr(p.status, kErrBlocks);
     }
     word_loads_arrive(bar);
     if (++next_slot == kSlots) next_slot = 0;
@@ -302,7 +314,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const uint32_t power = min(max(largest & 0x7f800000u, 27u << 23), 253u << 23);
-        const float down = __uint_as_float((254u << 23) - power);
+        const float down = __uint_as_float((254u << 23) - power) * p.q_sign;
         float up = __uint_as_float(power) * p.scale_log2;
         if (largest >= 0x7f800000u) up = __uint_as_float(0x7fc00000u);
 #pragma unroll
@@ -367,33 +379,54 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
     }
     release();
 
-    // Softmax: this thread has 8 tokens of two rows for each row tile.
-    const float v_log = log2f(v_scale);
-    const int64_t first_token = static_cast<int64_t>(at.tile) * kTileTokens + 16 * (octet >> 1) + (octet & 1);
+    // Softmax: this thread has 8 tokens of two rows for each row tile. With t = score + log2(v_scale), as long as no t is more
+    // than kStale above the row's `top`, nothing has to be agreed on between the threads of a row.
     const bool cut = (at.tile + int64_t{1}) * kTileTokens > static_cast<int64_t>(p.lengths[at.b]) - p.tokens + 1;
-    uint32_t p_hi[4][NT][2], p_lo[kSplit ? 4 : 1][kSplit ? NT : 1][2];
+    float factor[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) factor[n][e] = row_scale[n][e] * k_scale;
+    if (cut) {
+      const int64_t first_token = static_cast<int64_t>(at.tile) * kTileTokens + 16 * (octet >> 1) + (octet & 1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t seen = limit[n][e] - first_token;
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float& x = s[m][n][2 * h + e];
+              x = 4 * m + 2 * h < seen ? x * factor[n][e] : -INFINITY;  // (a masked position's scale may be anything)
+            }
+          factor[n][e] = 1.f;
+        }
+    }
+    const float v_log = __log2f(v_scale);
+    float best[NT][2];
+    bool higher = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float factor = row_scale[n][e] * k_scale;
-        float best = -INFINITY;
+        float x = s[0][n][e];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int i = 1; i < 8; ++i) x = fmaxf(x, s[i >> 1][n][2 * (i & 1) + e]);
+        best[n][e] = fmaf(x, factor[n][e], v_log);
+        higher |= best[n][e] > top[n][e] + kStale;
+      }
+    if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& x = s[m][n][2 * h + e];
-            x *= factor;
-            if (cut && first_token + 4 * m + 2 * h >= limit[n][e]) x = -INFINITY;
-            best = fmaxf(best, x);
-          }
-        best = best == -INFINITY ? best : best + v_log;  // (a masked position's scale may be anything)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-        if (__any_sync(0xffffffffu, best > top[n][e] + kStale)) {
-          const float higher = fmaxf(best, top[n][e]);
-          const float keep = higher == -INFINITY ? 1.f : fast_exp2(top[n][e] - higher);
-          top[n][e] = higher;
+        for (int e = 0; e < 2; ++e) {
+          float now = fmaxf(best[n][e], top[n][e]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+          const float keep = now == -INFINITY ? 1.f : fast_exp2(top[n][e] - now);
+          top[n][e] = now;
           sum[n][e] *= keep;
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) {
@@ -401,14 +434,20 @@ __global__ void __launch_bounds__(32 * kWarps, 1) cached_kernel(const CachedPara
             o[i][n][2 + e] *= keep;
           }
         }
-        const float shift = (top[n][e] == -INFINITY ? 0.f : top[n][e]) - kHeadroom;
+    }
+    uint32_t p_hi[4][NT][2], p_lo[kSplit ? 4 : 1][kSplit ? NT : 1][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float shift = kHeadroom - (top[n][e] == -INFINITY ? 0.f : top[n][e]);
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float& x = s[m][n][2 * h + e];
             const bool masked = cut && x == -INFINITY;
-            x = fast_exp2(x - shift);
+            x = fast_exp2(fmaf(x, factor[n][e], shift));
             sum[n][e] += x;
             x = masked ? 0.f : x * v_scale;
           }
@@ -597,9 +636,10 @@ CachedPlan plan_cached(const b200_cached_attention_desc& d, int sms) {
   plan.row_tiles = ceil_div(plan.rows, plan.tile);
   plan.pairs = d.batch * d.cache.heads * plan.row_tiles;
   // no more workers than the longest possible sequences have tiles
+  const int warps = d.cache.dim == 64 ? Ring<64>::kWarps : Ring<128>::kWarps;
   const int64_t most = plan.most = plan.pairs * (ceil_div(d.table_width * d.cache.block_tokens, kTileTokens) + 1);
   plan.grid = static_cast<int>(most < sms ? most : sms);
-  plan.workers = most < static_cast<int64_t>(plan.grid) * kWarps ? most : static_cast<int64_t>(plan.grid) * kWarps;
+  plan.workers = most < static_cast<int64_t>(plan.grid) * warps ? most : static_cast<int64_t>(plan.grid) * warps;
   return plan;
 }
 
@@ -622,7 +662,7 @@ cudaError_t launch_join(const CachedParams& p, const CachedPlan& plan, cudaStrea
 
 template <typename T, int D, int NT>
 int launch_cached(const CachedParams& p, const CachedPlan& plan, int sms, cudaStream_t s) {
-  cached_kernel<T, D, NT><<<plan.grid, 32 * kWarps, Ring<D>::kBytes, s>>>(p);
+  cached_kernel<T, D, NT><<<plan.grid, 32 * Ring<D>::kWarps, Ring<D>::kBytes, s>>>(p);
   const int code = check_launch();
   if (code) return finish(code);
   // A row has about workers / pairs partial results. With few pairs one warp would go over many of them.
@@ -702,7 +742,8 @@ extern "C" int b200_attention_cached(const b200_cached_attention_desc* desc, voi
   p.workers = static_cast<int32_t>(plan.workers);
   const int64_t vec = d.dtype == B200_F32 ? 4 : 8;
   p.q_vectors = aligned(d.q, 16) && d.q_batch % vec == 0 && d.q_token % vec == 0 && d.q_head % vec == 0;
-  p.scale_log2 = d.scale * kLog2e;
+  p.scale_log2 = d.scale == 0.f ? 1.f : fabsf(d.scale) * kLog2e;
+  p.q_sign = d.scale == 0.f ? 0.f : (d.scale < 0.f ? -1.f : 1.f);
   p.partial = static_cast<float*>(d.workspace);
   p.status = kernel_status_word();
   std::call_once(g_cached_attr_once[dev.device], [] {

@@ -32,26 +32,28 @@ struct PackedParams {
 
 // ------------------------------------------------------------------------- any type, any head size
 // One CTA takes 64 query rows of one head and goes over the keys in tiles of 64 with the running
-// maximum and sum of the softmax (f32 throughout, products by FFMA). 128 threads in an 8 x 16 grid:
-// a thread has 8 rows and 4 keys of the scores, and 8 rows and DP / 16 columns of the output
-// in registers; of the four LDS wavefronts per k the eight-row operand is a broadcast, so the
-// inner loops are bound by FFMA issue (32 a step) and not by shared memory. Operands
+// maximum and sum of the softmax (f32 throughout, products by FFMA). 256 threads in a 16 x 16 grid:
+// a thread has 4 rows and 4 keys of the scores, and 4 rows and DP / 16 columns of the output
+// in registers. Per step of the inner loops a warp reads three wavefronts of shared memory for 16 FFMA, so FFMA issue bounds
+// them (8 warps x 16 / 4 schedulers = 32 cycles against 24). K and V share a buffer (V is loaded when the scores
+// are done), which leaves room for two CTAs on an SM up to head size 96. Operands
 // lie transposed ([dim][row]) so that both are read as 16-byte vectors.
-constexpr int kTile = 64, kSimtThreads = 128, kPad = 4;
+constexpr int kTile = 64, kSimtThreads = 256, kPad = 4;
 
 template <int DP>
 constexpr size_t simt_smem_bytes() {
-  return (2 * DP * (kTile + kPad) + kTile * (DP + kPad) + kTile * (kTile + kPad)) * sizeof(float);
+  constexpr size_t keys = DP * (kTile + kPad), values = kTile * (DP + kPad);
+  return (DP * (kTile + kPad) + (keys > values ? keys : values) + kTile * (kTile + kPad)) * sizeof(float);
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kSimtThreads) packed_simt_kernel(const PackedParams p) {
+__global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_kernel(const PackedParams p) {
   extern __shared__ float smem[];
-  float* qt = smem;                           // [DP][64 + pad]
-  float* kt = qt + DP * (kTile + kPad);       // [DP][64 + pad]
-  float* vs = kt + DP * (kTile + kPad);       // [64][DP + pad]
-  float* ps = vs + kTile * (DP + kPad);       // [key][64 + pad]
-  constexpr int kStep = kTile + kPad, kVStep = DP + kPad, kCols = DP / 64;
+  constexpr int kStep = kTile + kPad, kVStep = DP + kPad, kCols = DP / 32;  // pairs of columns
+  float* qt = smem;                     // [DP][64 + pad]
+  float* ps = qt + DP * kStep;          // [key][64 + pad]
+  float* kt = ps + kTile * kStep;       // [DP][64 + pad]
+  float* vs = kt;                       // [64][DP + pad], when the scores are done
 
   const int head = blockIdx.y, dim = p.dim;
   // Tiles with many keys first (causal): a long sequence's last rows would otherwise start last.
@@ -80,42 +82,41 @@ __global__ void __launch_bounds__(kSimtThreads) packed_simt_kernel(const PackedP
   const T* k = static_cast<const T*>(p.k) + theirs.begin * p.k_row + kv_head * p.k_head;
   const T* v = static_cast<const T*>(p.v) + theirs.begin * p.v_row + kv_head * p.v_head;
 
-  for (int i = threadIdx.x; i < kTile * DP; i += kSimtThreads) {
-    const int r = i / DP, d = i % DP;
-    qt[d * kStep + r] = r < rows && d < dim ? Elem<T>::load(q + r * p.q_row + d) : 0.f;
-  }
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float top[8], total[8], acc[8][kCols * 4];
+  // A warp loads 32 consecutive channels of a row; past the end: zeros, whatever lies there.
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < kTile; r += 8)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+    for (int d = lane; d < DP; d += 32) qt[d * kStep + r] = r < rows && d < dim ? Elem<T>::load(q + r * p.q_row + d) : 0.f;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  float top[4], total[4], acc[4][kCols * 2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     top[i] = -INFINITY;
     total[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < kCols * 4; ++c) acc[i][c] = 0.f;
+    for (int c = 0; c < kCols * 2; ++c) acc[i][c] = 0.f;
   }
   for (int64_t key0 = 0; key0 < keys; key0 += kTile) {
     const int here = static_cast<int>(keys - key0 < kTile ? keys - key0 : kTile);
     __syncthreads();
-    for (int i = threadIdx.x; i < kTile * DP; i += kSimtThreads) {
-      const int r = i / DP, d = i % DP;
-      const bool in = r < here && d < dim;  // past the end: zeros, whatever lies there
-      kt[d * kStep + r] = in ? Elem<T>::load(k + (key0 + r) * p.k_row + d) : 0.f;
-      vs[r * kVStep + d] = in ? Elem<T>::load(v + (key0 + r) * p.v_row + d) : 0.f;
-    }
-    __syncthreads();
-    float s[8][4];
+#pragma unroll 2
+    for (int r = warp; r < kTile; r += 8)
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+      for (int d = lane; d < DP; d += 32)
+        kt[d * kStep + r] = r < here && d < dim ? Elem<T>::load(k + (key0 + r) * p.k_row + d) : 0.f;
+    __syncthreads();
+    float s[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int d = 0; d < DP; ++d) {
-      const float4 a0 = *reinterpret_cast<const float4*>(qt + d * kStep + ty * 8);
-      const float4 a1 = *reinterpret_cast<const float4*>(qt + d * kStep + ty * 8 + 4);
+      const float4 a4 = *reinterpret_cast<const float4*>(qt + d * kStep + ty * 4);
       const float4 b = *reinterpret_cast<const float4*>(kt + d * kStep + tx * 4);
-      const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      const float a[4] = {a4.x, a4.y, a4.z, a4.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         s[i][0] = fmaf(a[i], b.x, s[i][0]);
         s[i][1] = fmaf(a[i], b.y, s[i][1]);
         s[i][2] = fmaf(a[i], b.z, s[i][2]);
@@ -125,8 +126,8 @@ __global__ void __launch_bounds__(kSimtThreads) packed_simt_kernel(const PackedP
     // Whether some row of the tile sees only a part of these keys.
     const bool cut = p.causal && row0 + shift < key0 + here;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t limit = p.causal ? row0 + ty * 8 + i + shift - key0 : here;
+    for (int i = 0; i < 4; ++i) {
+      const int64_t limit = p.causal ? row0 + ty * 4 + i + shift - key0 : here;
       float best = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -142,49 +143,55 @@ __global__ void __launch_bounds__(kSimtThreads) packed_simt_kernel(const PackedP
       top[i] = best;
       total[i] *= keep;
 #pragma unroll
-      for (int c = 0; c < kCols * 4; ++c) acc[i][c] *= keep;
+      for (int c = 0; c < kCols * 2; ++c) acc[i][c] *= keep;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         s[i][j] = fast_exp2(s[i][j] - base);
         total[i] += s[i][j];
-        ps[(tx * 4 + j) * kStep + ty * 8 + i] = s[i][j];
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<float4*>(ps + (tx * 4 + j) * kStep + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
     __syncthreads();
+#pragma unroll 2
+    for (int r = warp; r < kTile; r += 8)
+#pragma unroll
+      for (int d = lane; d < DP; d += 32)
+        vs[r * kVStep + d] = r < here && d < dim ? Elem<T>::load(v + (key0 + r) * p.v_row + d) : 0.f;
+    __syncthreads();
+#pragma unroll 4
     for (int key = 0; key < here; ++key) {
-      const float4 a0 = *reinterpret_cast<const float4*>(ps + key * kStep + ty * 8);
-      const float4 a1 = *reinterpret_cast<const float4*>(ps + key * kStep + ty * 8 + 4);
-      const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      const float4 a4 = *reinterpret_cast<const float4*>(ps + key * kStep + ty * 4);
+      const float a[4] = {a4.x, a4.y, a4.z, a4.w};
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
-        const float4 b = *reinterpret_cast<const float4*>(vs + key * kVStep + c * 64 + tx * 4);
+        const float2 b = *reinterpret_cast<const float2*>(vs + key * kVStep + c * 32 + tx * 2);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           // A masked value must not be read as 0 * value: it may be an infinity or NaN.
-          if (cut && key0 + key >= row0 + ty * 8 + i + shift) continue;
-          acc[i][c * 4] = fmaf(a[i], b.x, acc[i][c * 4]);
-          acc[i][c * 4 + 1] = fmaf(a[i], b.y, acc[i][c * 4 + 1]);
-          acc[i][c * 4 + 2] = fmaf(a[i], b.z, acc[i][c * 4 + 2]);
-          acc[i][c * 4 + 3] = fmaf(a[i], b.w, acc[i][c * 4 + 3]);
+          if (cut && key0 + key >= row0 + ty * 4 + i + shift) continue;
+          acc[i][c * 2] = fmaf(a[i], b.x, acc[i][c * 2]);
+          acc[i][c * 2 + 1] = fmaf(a[i], b.y, acc[i][c * 2 + 1]);
         }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) total[i] += __shfl_xor_sync(0xffffffffu, total[i], o);
-    const int r = ty * 8 + i;
+    const int r = ty * 4 + i;
     if (r >= rows) continue;
-    const bool none = p.causal ? row0 + r + shift <= 0 || theirs.count == 0 : theirs.count == 0;
+    const bool none = theirs.count == 0 || (p.causal && row0 + r + shift <= 0);
     const float inv = none ? 0.f : 1.f / total[i];
     T* dst = out + ((mine.begin + row0 + r) * p.heads + head) * dim;
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = c * 64 + tx * 4 + j;
-        if (d < dim) Elem<T>::store(dst + d, none ? 0.f : acc[i][c * 4 + j] * inv);
+      for (int j = 0; j < 2; ++j) {
+        const int d = c * 32 + tx * 2 + j;
+        if (d < dim) Elem<T>::store(dst + d, none ? 0.f : acc[i][c * 2 + j] * inv);
       }
   }
 }
@@ -197,22 +204,30 @@ void launch_simt(const PackedParams& p, cudaStream_t s) {
   packed_simt_kernel<T, DP><<<grid, kSimtThreads, simt_smem_bytes<DP>(), s>>>(p);
 }
 
+template <typename T, int DP>
+void simt_attribute() {
+  cudaFuncSetAttribute(packed_simt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       static_cast<int>(simt_smem_bytes<DP>()));
+}
 template <typename T>
 void simt_attributes() {
-  cudaFuncSetAttribute(packed_simt_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       static_cast<int>(simt_smem_bytes<64>()));
-  cudaFuncSetAttribute(packed_simt_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       static_cast<int>(simt_smem_bytes<128>()));
-  cudaFuncSetAttribute(packed_simt_kernel<T, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       static_cast<int>(simt_smem_bytes<256>()));
+  simt_attribute<T, 64>();
+  simt_attribute<T, 96>();
+  simt_attribute<T, 128>();
+  simt_attribute<T, 192>();
+  simt_attribute<T, 256>();
 }
 
 template <typename T>
 void launch_simt_any(const PackedParams& p, cudaStream_t s) {
   if (p.dim <= 64)
     launch_simt<T, 64>(p, s);
+  else if (p.dim <= 96)
+    launch_simt<T, 96>(p, s);
   else if (p.dim <= 128)
     launch_simt<T, 128>(p, s);
+  else if (p.dim <= 192)
+    launch_simt<T, 192>(p, s);
   else
     launch_simt<T, 256>(p, s);
 }

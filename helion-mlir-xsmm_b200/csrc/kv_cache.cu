@@ -110,13 +110,13 @@ struct AppendParams {
   int32_t* status;
 };
 
-// A thread holds 8 values of each of 4 consecutive tokens. Threads of a warp go along the head first
-// for K (8 code bytes of a token next to each other) and along the tokens first for V (4 codes of a
-// channel in one word, the words of a channel next to each other), so both leave in whole sectors. A CTA is one chain of
-// dependent loads (lengths, then its values and the table, then the block's scale and codes): what counts is how many
-// are on an SM, so registers are held to four CTAs of 256 threads.
-template <typename T, bool is_v>
-__device__ __forceinline__ void append_block(const AppendParams& p) {
+// Which block a CTA writes, and the slots [first, stop) of it that are new; `row` is the packed row of slot 0.
+struct AppendPlace {
+  int32_t sequence;
+  int64_t page, row;
+  int first, stop;
+};
+__device__ __forceinline__ bool find_append(const AppendParams& p, AppendPlace& at) {
   const Cache& c = p.cache;
   auto new_rows = [&](int32_t b) {
     if (p.offsets) return rows_of(p.offsets, b, p.rows, p.status);
@@ -128,20 +128,40 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
       const int64_t n = new_rows(b).count, length = max(p.lengths[b], 0);
       return n == 0 ? int64_t{0} : ((length + n - 1) >> c.token_bits) - (length >> c.token_bits) + 1;
     });
-  if (piece.sequence < 0) return;
+  if (piece.sequence < 0) return false;
   const Rows rows = new_rows(piece.sequence);
   const int64_t length = max(p.lengths[piece.sequence], 0);
-  const int64_t page = (length >> c.token_bits) + piece.index;
-  const int64_t start = page << c.token_bits;
-  const int first = static_cast<int>(max(length, start) - start);  // slots [first, stop) are new
-  const int stop = static_cast<int>(min(length + rows.count, start + c.tokens) - start);
+  at.sequence = piece.sequence;
+  at.page = (length >> c.token_bits) + piece.index;
+  const int64_t start = at.page << c.token_bits;
+  at.first = static_cast<int>(max(length, start) - start);
+  at.stop = static_cast<int>(min(length + rows.count, start + c.tokens) - start);
+  at.row = rows.begin + start - length;
+  return true;
+}
+// The block's scale from the largest new magnitude (its bits) and the scale before.
+__device__ __forceinline__ float new_scale(uint32_t largest, float before, bool& finite) {
+  finite = largest < kInfBits && before == before;
+  const float s = fmaxf(fmaxf(__fdiv_rn(__uint_as_float(largest), 127.f), kSmallestScale), before);
+  return finite ? s : __uint_as_float(0x7fc00000u);
+}
 
+// A thread holds 8 values of each of 4 consecutive tokens. Threads of a warp go along the head first
+// for K (8 code bytes of a token next to each other) and along the tokens first for V (4 codes of a
+// channel in one word, the words of a channel next to each other), so both leave in whole sectors. A CTA is one chain of
+// dependent loads (lengths, then its values and the table, then the block's scale and codes): what counts is how many
+// are on an SM, so registers are held to four CTAs of 256 threads.
+template <typename T, bool is_v>
+__device__ __forceinline__ void append_block(const AppendParams& p) {
+  const Cache& c = p.cache;
+  AppendPlace place;
+  if (!find_append(p, place)) return;
+  const int first = place.first, stop = place.stop;
   const int head = blockIdx.y, parts = c.dim / 8, groups = c.tokens / 4;
   const int part = is_v ? threadIdx.x / groups : threadIdx.x % parts;
   const int slot0 = 4 * (is_v ? threadIdx.x % groups : threadIdx.x / parts);
   const int64_t step = is_v ? p.v_row : p.k_row;
-  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + part * 8 + (rows.begin + start - length) * step +
-                 head * (is_v ? p.v_head : p.k_head);
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + part * 8 + place.row * step + head * (is_v ? p.v_head : p.k_head);
   auto is_new = [&](int j) { return slot0 + j >= first && slot0 + j < stop; };
   const bool any_new = slot0 + 4 > first && slot0 < stop, all_new = slot0 >= first && slot0 + 4 <= stop;
   const bool any_old = slot0 < first;
@@ -154,7 +174,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
     else
       here[j].clear();
   }
-  const int64_t block = block_of(c, p.table, piece.sequence, page, p.status);
+  const int64_t block = block_of(c, p.table, place.sequence, place.page, p.status);
   if (block < 0) return;
   float* scale = (is_v ? c.v_scales : c.k_scales) + block * c.heads + head;
   const float before = first > 0 ? *scale : 0.f;
@@ -186,9 +206,8 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
   __syncthreads();
   largest = warp_largest[0];
   for (unsigned w = 1; w < blockDim.x / 32; ++w) largest = max(largest, warp_largest[w]);
-  float s = fmaxf(fmaxf(__fdiv_rn(__uint_as_float(largest), 127.f), kSmallestScale), before);
-  const bool finite = largest < kInfBits && before == before;
-  if (!finite) s = __uint_as_float(0x7fc00000u);
+  bool finite;
+  const float s = new_scale(largest, before, finite);
   if (threadIdx.x == 0 && !(s == before)) *scale = s;  // (every thread has read it before the barrier)
 
   const bool grew = finite && first > 0 && s > before;
@@ -246,6 +265,112 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) kv_append_kernel(
     append_block<T, true>(p);
   else
     append_block<T, false>(p);
+}
+
+// The same write when the blocks get few tokens each (single tokens of many sequences): a warp for each (block, head,
+// K or V), whose lanes hold dim / 32 channels of a token. A CTA of the kernel above would be up to 256 threads for
+// one token (128 tokens into blocks of 64: 23.5 us, and 5.3 here).
+template <typename T, int PER>
+__device__ __forceinline__ void load_channels(const T* p, float (&v)[PER]) {  // dim / 32 = 2 or 4 channels
+  if (sizeof(T) * PER == 16) {
+    const uint4 w = ld_stream16(p);
+    v[0] = __uint_as_float(w.x);
+    v[1] = __uint_as_float(w.y);
+    v[PER - 2] = __uint_as_float(w.z);
+    v[PER - 1] = __uint_as_float(w.w);
+  } else if (sizeof(T) == 4) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    v[0] = __uint_as_float(w.x);
+    v[1] = __uint_as_float(w.y);
+  } else if (PER == 4) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    v[0] = __uint_as_float(w.x << 16);
+    v[1] = __uint_as_float(w.x & 0xffff0000u);
+    v[PER - 2] = __uint_as_float(w.y << 16);
+    v[PER - 1] = __uint_as_float(w.y & 0xffff0000u);
+  } else {
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p));
+    v[0] = __uint_as_float(w << 16);
+    v[1] = __uint_as_float(w & 0xffff0000u);
+  }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(256) kv_append_few_kernel(const AppendParams p) {
+  const Cache& c = p.cache;
+  const int lane = threadIdx.x & 31;
+  const int task = blockIdx.y * 8 + (threadIdx.x >> 5), head = task >> 1;
+  const bool is_v = task & 1;
+  AppendPlace at;
+  if (!find_append(p, at) || head >= c.heads) return;
+  const int first = at.first, stop = at.stop;
+  const int64_t step = is_v ? p.v_row : p.k_row;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + at.row * step + head * (is_v ? p.v_head : p.k_head) + lane * PER;
+  float x[PER];
+  load_channels<T, PER>(src + first * step, x);  // of the first token: often the only one
+  const int64_t block = block_of(c, p.table, at.sequence, at.page, p.status);
+  if (block < 0) return;
+  float* scale = (is_v ? c.v_scales : c.k_scales) + block * c.heads + head;
+  const float before = first > 0 ? *scale : 0.f;
+  uint32_t largest = 0;
+  for (int slot = first; slot < stop; ++slot) {
+    float y[PER];
+    if (slot == first) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) y[i] = x[i];
+    } else {
+      load_channels<T, PER>(src + slot * step, y);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) largest = max(largest, __float_as_uint(y[i]) & 0x7fffffffu);
+  }
+  largest = __reduce_max_sync(0xffffffffu, largest);
+  bool finite;
+  const float s = new_scale(largest, before, finite);
+  if (lane == 0 && !(s == before)) *scale = s;
+  int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
+  if (finite && first > 0 && s > before) {
+    const float ratio = __fdiv_rn(before, s);
+    const int words = is_v ? (first + 3) / 4 : c.dim / 4;  // of a channel's old tokens, or of a token
+    const int rows = is_v ? c.dim : first;
+    for (int i = lane; i < rows * words; i += 32) {
+      const int row = i / words, word = i - row * words;
+      uint32_t* where = reinterpret_cast<uint32_t*>(codes + row * (is_v ? c.tokens : c.dim) + word * 4);
+      const uint32_t old = *where;
+      uint32_t w = old;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!is_v || word * 4 + e < first) w = with_code(w, e, rescaled(code_value(w, e), before, s, ratio));
+      *where = w;
+    }
+    __syncwarp();  // a word of V may hold new tokens too: they are written after it
+  }
+  const float inv = __frcp_rn(s);
+  for (int slot = first; slot < stop; ++slot) {
+    if (slot > first) load_channels<T, PER>(src + slot * step, x);
+    bool near_tie = false;
+    float code[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) code[i] = quotient(x[i], s, inv, near_tie);
+    if (near_tie) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) code[i] = quotient_at_tie(x[i], s, code[i]);
+    }
+    if (is_v) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        codes[(lane * PER + i) * c.tokens + slot] = static_cast<int8_t>(finite ? __float_as_uint(code[i]) & 255 : 0);
+    } else {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) w = with_code(w, i, finite ? code[i] : kWhole);
+      int8_t* where = codes + slot * c.dim + lane * PER;
+      if (PER == 4)
+        *reinterpret_cast<uint32_t*>(where) = w;
+      else
+        *reinterpret_cast<uint16_t*>(where) = static_cast<uint16_t>(w);
+    }
+  }
 }
 
 struct ReadParams {
@@ -352,6 +477,10 @@ int heads_for(int64_t pieces, int heads, int sms) {
   return each;
 }
 
+// New tokens a sequence, on average, up to which a warp takes a block. 64 sequences: 3 tokens each 8.4 against 13.9 us (blocks
+// of 64), 7 tokens each 15.7 against 15.3 and, in blocks of 16, 10.7 against 8.1.
+constexpr int64_t kFewTokens = 4;
+
 bool table_ok(const int32_t* table, int64_t batch, int64_t stride, int64_t width) {
   return width >= 0 && width <= INT32_MAX && (batch <= 1 || stride >= width) && (table || width == 0);
 }
@@ -395,9 +524,21 @@ extern "C" int b200_kv_append(const b200_kv_append_desc* desc, void* stream) {
   p.status = kernel_status_word();
   // n new tokens touch at most (n - 2) / tokens + 2 blocks; one token each, one block each
   const int64_t pieces = !d.offsets && d.rows == d.batch ? d.batch : d.rows / d.cache.block_tokens + 2 * d.batch;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (d.rows <= kFewTokens * d.batch) {
+    const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(ceil_div(2 * d.cache.heads, 8)));
+    if (d.dtype == B200_F32 && d.cache.dim == 64)
+      kv_append_few_kernel<float, 2><<<grid, 256, 0, s>>>(p);
+    else if (d.dtype == B200_F32)
+      kv_append_few_kernel<float, 4><<<grid, 256, 0, s>>>(p);
+    else if (d.cache.dim == 64)
+      kv_append_few_kernel<__nv_bfloat16, 2><<<grid, 256, 0, s>>>(p);
+    else
+      kv_append_few_kernel<__nv_bfloat16, 4><<<grid, 256, 0, s>>>(p);
+    return launched();
+  }
   const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(d.cache.heads), 2);
   const unsigned threads = static_cast<unsigned>(d.cache.block_tokens / 4 * (d.cache.dim / 8));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d.dtype == B200_F32)
     kv_append_kernel<float><<<grid, threads, 0, s>>>(p);
   else
