@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "sequences.cuh"
 #include "umma_ptx.cuh"
@@ -26,6 +27,7 @@ struct PackedParams {
   const int32_t *offsets, *k_offsets;
   int32_t batch, heads, group, dim;  // group: query heads that share a key/value head
   int32_t causal;
+  int32_t vectors;   // f32 rows can be copied in 16-byte pieces
   float scale_log2;  // scale * log2(e)
   int32_t* status;
 };
@@ -34,26 +36,50 @@ struct PackedParams {
 // One CTA takes 64 query rows of one head and goes over the keys in tiles of 64 with the running
 // maximum and sum of the softmax (f32 throughout, products by FFMA). 256 threads in a 16 x 16 grid:
 // a thread has 4 rows and 4 keys of the scores, and 4 rows and DP / 16 columns of the output
-// in registers. Per step of the inner loops a warp reads three wavefronts of shared memory for 16 FFMA, so FFMA issue bounds
-// them (8 warps x 16 / 4 schedulers = 32 cycles against 24). K and V share a buffer (V is loaded when the scores
-// are done), which leaves room for two CTAs on an SM up to head size 96. Operands
-// lie transposed ([dim][row]) so that both are read as 16-byte vectors.
+// in registers. For the scores both operands are read along the head, four channels at a time: 8 LDS.128 for 64 FFMA, 24
+// wavefronts for 32 cycles of FFMA a channel, so FFMA issue bounds the inner loops; rows are DP + 4 floats
+// apart, which puts the 16-byte pieces of consecutive rows on different banks. The tile of V comes in (cp.async) while the scores are
+// computed, the next tile of K while P V is; two CTAs fit on an SM up to head size 96.
 constexpr int kTile = 64, kSimtThreads = 256, kPad = 4;
 
 template <int DP>
 constexpr size_t simt_smem_bytes() {
-  constexpr size_t keys = DP * (kTile + kPad), values = kTile * (DP + kPad);
-  return (DP * (kTile + kPad) + (keys > values ? keys : values) + kTile * (kTile + kPad)) * sizeof(float);
+  return (3 * kTile * (DP + kPad) + kTile * (kTile + kPad)) * sizeof(float);
+}
+
+// 64 rows of `dim` values into rows of DP + 4 floats; rows from `count` on and channels from dim on are zeros, whatever lies
+// there. Complete after the copies have been waited for (a barrier follows either form).
+template <typename T, int DP>
+__device__ __forceinline__ void simt_load(float* dst, const T* src, int64_t row_step, int count, int dim, bool vectors) {
+  if (sizeof(T) == 4 && vectors) {
+    for (int i = threadIdx.x; i < kTile * (DP / 4); i += kSimtThreads) {
+      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+      const bool in = r < count && d < dim;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * (DP + kPad) + d)),
+                   "l"(in ? src + r * row_step + d : src), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 2
+  for (int r = warp; r < kTile; r += 8)
+#pragma unroll
+    for (int d = lane; d < DP; d += 32) dst[r * (DP + kPad) + d] = r < count && d < dim ? Elem<T>::load(src + r * row_step + d) : 0.f;
+}
+__device__ __forceinline__ void simt_loaded() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_kernel(const PackedParams p) {
   extern __shared__ float smem[];
-  constexpr int kStep = kTile + kPad, kVStep = DP + kPad, kCols = DP / 32;  // pairs of columns
-  float* qt = smem;                     // [DP][64 + pad]
-  float* ps = qt + DP * kStep;          // [key][64 + pad]
-  float* kt = ps + kTile * kStep;       // [DP][64 + pad]
-  float* vs = kt;                       // [64][DP + pad], when the scores are done
+  constexpr int kStep = DP + kPad, kPStep = kTile + kPad, kCols = DP / 32;  // kCols: pairs of columns
+  float* qs = smem;                  // [64][DP + pad]
+  float* ks = qs + kTile * kStep;
+  float* vs = ks + kTile * kStep;
+  float* ps = vs + kTile * kStep;    // [key][64 + pad]
 
   const int head = blockIdx.y, dim = p.dim;
   // Tiles with many keys first (causal): a long sequence's last rows would otherwise start last.
@@ -82,11 +108,8 @@ __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_ke
   const T* k = static_cast<const T*>(p.k) + theirs.begin * p.k_row + kv_head * p.k_head;
   const T* v = static_cast<const T*>(p.v) + theirs.begin * p.v_row + kv_head * p.v_head;
 
-  // A warp loads 32 consecutive channels of a row; past the end: zeros, whatever lies there.
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < kTile; r += 8)
-#pragma unroll
-    for (int d = lane; d < DP; d += 32) qt[d * kStep + r] = r < rows && d < dim ? Elem<T>::load(q + r * p.q_row + d) : 0.f;
+  simt_load<T, DP>(qs, q, p.q_row, rows, dim, p.vectors);
+  if (keys > 0) simt_load<T, DP>(ks, k, p.k_row, static_cast<int>(keys < kTile ? keys : kTile), dim, p.vectors);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   float top[4], total[4], acc[4][kCols * 2];
 #pragma unroll
@@ -98,30 +121,25 @@ __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_ke
   }
   for (int64_t key0 = 0; key0 < keys; key0 += kTile) {
     const int here = static_cast<int>(keys - key0 < kTile ? keys - key0 : kTile);
-    __syncthreads();
-#pragma unroll 2
-    for (int r = warp; r < kTile; r += 8)
-#pragma unroll
-      for (int d = lane; d < DP; d += 32)
-        kt[d * kStep + r] = r < here && d < dim ? Elem<T>::load(k + (key0 + r) * p.k_row + d) : 0.f;
-    __syncthreads();
+    simt_loaded();  // K (and Q); V of the last tile has been read
+    simt_load<T, DP>(vs, v + key0 * p.v_row, p.v_row, here, dim, p.vectors);
     float s[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 8
-    for (int d = 0; d < DP; ++d) {
-      const float4 a4 = *reinterpret_cast<const float4*>(qt + d * kStep + ty * 4);
-      const float4 b = *reinterpret_cast<const float4*>(kt + d * kStep + tx * 4);
-      const float a[4] = {a4.x, a4.y, a4.z, a4.w};
+#pragma unroll 2
+    for (int d = 0; d < DP; d += 4) {
+      float4 a[4], b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i][0] = fmaf(a[i], b.x, s[i][0]);
-        s[i][1] = fmaf(a[i], b.y, s[i][1]);
-        s[i][2] = fmaf(a[i], b.z, s[i][2]);
-        s[i][3] = fmaf(a[i], b.w, s[i][3]);
-      }
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * kStep + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kStep + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
     }
     // Whether some row of the tile sees only a part of these keys.
     const bool cut = p.causal && row0 + shift < key0 + here;
@@ -131,7 +149,7 @@ __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_ke
       float best = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int key = tx * 4 + j;
+        const int key = tx + 16 * j;
         s[i][j] = key < here && key < limit ? s[i][j] * p.scale_log2 : -INFINITY;
         best = fmaxf(best, s[i][j]);
       }
@@ -152,30 +170,37 @@ __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_ke
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4*>(ps + (tx * 4 + j) * kStep + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
-    __syncthreads();
-#pragma unroll 2
-    for (int r = warp; r < kTile; r += 8)
+      *reinterpret_cast<float4*>(ps + (tx + 16 * j) * kPStep + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    simt_loaded();  // V and P; K has been read
+    if (key0 + kTile < keys)
+      simt_load<T, DP>(ks, k + (key0 + kTile) * p.k_row, p.k_row, static_cast<int>(keys - key0 - kTile < kTile ? keys - key0 - kTile : kTile),
+                       dim, p.vectors);
+    // A masked value must not be read as 0 * value (it may be an infinity or NaN): where the mask cuts the tile, row i
+    // takes the keys below seen[i].
+    auto add_values = [&](auto masked) {
+      int seen[4];
 #pragma unroll
-      for (int d = lane; d < DP; d += 32)
-        vs[r * kVStep + d] = r < here && d < dim ? Elem<T>::load(v + (key0 + r) * p.v_row + d) : 0.f;
-    __syncthreads();
+      for (int i = 0; i < 4; ++i) seen[i] = static_cast<int>(min(row0 + ty * 4 + i + shift - key0, int64_t{kTile}));
 #pragma unroll 4
-    for (int key = 0; key < here; ++key) {
-      const float4 a4 = *reinterpret_cast<const float4*>(ps + key * kStep + ty * 4);
-      const float a[4] = {a4.x, a4.y, a4.z, a4.w};
+      for (int key = 0; key < here; ++key) {
+        const float4 a4 = *reinterpret_cast<const float4*>(ps + key * kPStep + ty * 4);
+        const float a[4] = {a4.x, a4.y, a4.z, a4.w};
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const float2 b = *reinterpret_cast<const float2*>(vs + key * kVStep + c * 32 + tx * 2);
+        for (int c = 0; c < kCols; ++c) {
+          const float2 b = *reinterpret_cast<const float2*>(vs + key * kStep + c * 32 + tx * 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // A masked value must not be read as 0 * value: it may be an infinity or NaN.
-          if (cut && key0 + key >= row0 + ty * 4 + i + shift) continue;
-          acc[i][c * 2] = fmaf(a[i], b.x, acc[i][c * 2]);
-          acc[i][c * 2 + 1] = fmaf(a[i], b.y, acc[i][c * 2 + 1]);
+          for (int i = 0; i < 4; ++i) {
+            if (decltype(masked)::value && key >= seen[i]) continue;
+            acc[i][c * 2] = fmaf(a[i], b.x, acc[i][c * 2]);
+            acc[i][c * 2 + 1] = fmaf(a[i], b.y, acc[i][c * 2 + 1]);
+          }
         }
       }
-    }
+    };
+    if (cut)
+      add_values(std::true_type{});
+    else
+      add_values(std::false_type{});
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -781,6 +806,8 @@ extern "C" int b200_attention_packed(const b200_packed_attention_desc* desc, voi
   p.group = static_cast<int32_t>(d.heads / d.kv_heads);
   p.dim = static_cast<int32_t>(d.dim);
   p.causal = d.causal;
+  const int64_t strides = d.q_row | d.q_head | d.k_row | d.k_head | d.v_row | d.v_head | d.dim;
+  p.vectors = strides % 4 == 0 && aligned(d.q, 16) && aligned(d.k, 16) && aligned(d.v, 16);
   p.scale_log2 = d.scale * kLog2e;
   p.status = kernel_status_word();
 
