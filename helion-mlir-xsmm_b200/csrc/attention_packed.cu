@@ -9,7 +9,6 @@
 #include <math.h>
 
 #include <mutex>
-#include <type_traits>
 
 #include "sequences.cuh"
 #include "umma_ptx.cuh"
@@ -27,61 +26,152 @@ struct PackedParams {
   const int32_t *offsets, *k_offsets;
   int32_t batch, heads, group, dim;  // group: query heads that share a key/value head
   int32_t causal;
-  int32_t vectors;   // f32 rows can be copied in 16-byte pieces
+  int32_t vectors;   // rows can be read four values at a time
   float scale_log2;  // scale * log2(e)
   int32_t* status;
 };
 
 // ------------------------------------------------------------------------- any type, any head size
-// One CTA takes 64 query rows of one head and goes over the keys in tiles of 64 with the running
-// maximum and sum of the softmax (f32 throughout, products by FFMA). 256 threads in a 16 x 16 grid:
-// a thread has 4 rows and 4 keys of the scores, and 4 rows and DP / 16 columns of the output
-// in registers. For the scores both operands are read along the head, four channels at a time: 8 LDS.128 for 64 FFMA, 24
-// wavefronts for 32 cycles of FFMA a channel, so FFMA issue bounds the inner loops; rows are DP + 4 floats
-// apart, which puts the 16-byte pieces of consecutive rows on different banks. The tile of V comes in (cp.async) while the scores are
-// computed, the next tile of K while P V is; two CTAs fit on an SM up to head size 96.
-constexpr int kTile = 64, kSimtThreads = 256, kPad = 4;
-
-template <int DP>
-constexpr size_t simt_smem_bytes() {
-  return (3 * kTile * (DP + kPad) + kTile * (kTile + kPad)) * sizeof(float);
+// Values that a row does not see must not reach it, but the tensor core multiplies them by P = 0, and 0 * infinity is NaN. So
+// a row whose result is not finite looks whether a value that is not finite lies among the keys that were read and not
+// seen ([sees, read)), and one thread computes its columns [from, to) again if so (`always`: in any case).
+template <typename T>
+__device__ __forceinline__ void packed_row_again(const PackedParams& p, const T* q, const T* k, const T* v, int64_t sees, int64_t read,
+                                                 bool always, int from, int to, T* dst) {
+  bool touched = always;
+  for (int64_t j = sees; j < read && !touched; ++j)
+    for (int d = from; d < to; ++d) touched |= !isfinite(Elem<T>::load(v + j * p.v_row + d));
+  if (!touched) return;  // the row itself is not finite
+#pragma unroll 1
+  for (int chunk = from; chunk < to; chunk += 32) {
+    float acc[32], top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+#pragma unroll 1
+    for (int64_t j = 0; j < sees; ++j) {
+      float s = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < p.dim; ++d) s = fmaf(Elem<T>::load(q + d), Elem<T>::load(k + j * p.k_row + d), s);
+      s *= p.scale_log2;
+      const float best = fmaxf(top, s), base = best == -INFINITY ? 0.f : best;
+      const float keep = fast_exp2(top - base), weight = fast_exp2(s - base);
+      top = best;
+      total = fmaf(total, keep, weight);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (chunk + i < to) acc[i] = fmaf(weight, Elem<T>::load(v + j * p.v_row + chunk + i), acc[i] * keep);
+    }
+    const float inv = 1.f / total;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (chunk + i < to) Elem<T>::store(dst + chunk + i, acc[i] * inv);
+  }
 }
 
-// 64 rows of `dim` values into rows of DP + 4 floats; rows from `count` on and channels from dim on are zeros, whatever lies
-// there. Complete after the copies have been waited for (a barrier follows either form).
+// One CTA takes 64 query rows of one head and goes over the keys in tiles, with the running maximum and sum of the
+// softmax in f32. Eight warps: four runs of 16 rows, two halves of each tile's keys, joined at the end. The products are
+// mma m16n8k16 on bf16 pieces: an f32 value is the sum of three (8 + 8 + 8 bits, the exponent range of f32, so nothing
+// has to be scaled), and a product the six of their products that reach 2^-24; Q, K, V and P alike. That is f32's own
+// accuracy at six instructions; FFMA tiles of 64 x 64 stood still on shared memory at a third of FFMA's rate (five
+// sequences of 300, 6 heads of 80: 84 us; one of 4096, 8 heads of 64: 775 us). bf16 values are one piece.
+constexpr int kTile = 64, kMmaThreads = 256;
+
 template <typename T, int DP>
-__device__ __forceinline__ void simt_load(float* dst, const T* src, int64_t row_step, int count, int dim, bool vectors) {
-  if (sizeof(T) == 4 && vectors) {
-    for (int i = threadIdx.x; i < kTile * (DP / 4); i += kSimtThreads) {
-      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-      const bool in = r < count && d < dim;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * (DP + kPad) + d)),
-                   "l"(in ? src + r * row_step + d : src), "r"(in ? 16 : 0)
-                   : "memory");
-    }
+struct MmaTile {
+  static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int kKeys = sizeof(T) == 4 && DP > 128 ? 32 : 64;  // of a tile: as many as leave room in shared memory
+  static constexpr int kStep = DP + 8;  // of a row: the 16-byte pieces of eight rows on different banks
+  static constexpr uint32_t kQPiece = kTile * kStep, kKeyPiece = kKeys * kStep;  // elements
+  static constexpr size_t kTiles = kPieces * (kQPiece + 2 * kKeyPiece) * 2;
+  static constexpr size_t kJoin = 4 * 32 * (DP / 2 + 4) * 4;  // what four warps hand over at the end
+  static constexpr size_t kBytes = kTiles > kJoin ? kTiles : kJoin;
+};
+
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two values as bf16 pairs: one, rounded to the nearest, or three, each the upper 16 bits of what the ones before leave over
+// (cut off, not rounded: nothing overflows, and the last takes the rest exactly).
+template <int PIECES>
+__device__ __forceinline__ void to_pieces(float lo, float hi, uint32_t (&piece)[PIECES]) {
+  if (PIECES == 1) {
+    piece[0] = pack_bf16x2(lo, hi);
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll 2
-  for (int r = warp; r < kTile; r += 8)
 #pragma unroll
-    for (int d = lane; d < DP; d += 32) dst[r * (DP + kPad) + d] = r < count && d < dim ? Elem<T>::load(src + r * row_step + d) : 0.f;
+  for (int i = 0; i < PIECES; ++i) {
+    const uint32_t a = __float_as_uint(lo), b = __float_as_uint(hi);
+    piece[i] = __byte_perm(a, b, 0x7632);
+    lo -= __uint_as_float(a & 0xffff0000u);
+    hi -= __uint_as_float(b & 0xffff0000u);
+  }
 }
-__device__ __forceinline__ void simt_loaded() {
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();
+
+// `rows` rows of `dim` values as pieces into shared memory; rows from `count` on and channels from dim on are zeros, whatever
+// lies there.
+template <typename T, int DP>
+__device__ __forceinline__ void mma_load(__nv_bfloat16* dst, uint32_t piece_step, const T* src, int64_t row_step, int rows, int count,
+                                         int dim, bool vectors) {
+  using Tile = MmaTile<T, DP>;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * (DP / 4); i += kMmaThreads) {
+    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < count && d < dim) {
+      const T* at = src + r * row_step + d;
+      if (vectors) {  // dim is a multiple of four then
+        if (sizeof(T) == 4) {
+          unpack16(ld_plain16(at), x);
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(at);
+          x[0] = __uint_as_float(w.x << 16);
+          x[1] = __uint_as_float(w.x & 0xffff0000u);
+          x[2] = __uint_as_float(w.y << 16);
+          x[3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < dim) x[e] = Elem<T>::load(at + e);
+      }
+    }
+    uint32_t lo[Tile::kPieces], hi[Tile::kPieces];
+    to_pieces<Tile::kPieces>(x[0], x[1], lo);
+    to_pieces<Tile::kPieces>(x[2], x[3], hi);
+#pragma unroll
+    for (int e = 0; e < Tile::kPieces; ++e)
+      *reinterpret_cast<uint2*>(dst + e * piece_step + r * Tile::kStep + d) = make_uint2(lo[e], hi[e]);
+  }
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_kernel(const PackedParams p) {
-  extern __shared__ float smem[];
-  constexpr int kStep = DP + kPad, kPStep = kTile + kPad, kCols = DP / 32;  // kCols: pairs of columns
-  float* qs = smem;                  // [64][DP + pad]
-  float* ks = qs + kTile * kStep;
-  float* vs = ks + kTile * kStep;
-  float* ps = vs + kTile * kStep;    // [key][64 + pad]
+__global__ void __launch_bounds__(kMmaThreads, DP <= 96 || (sizeof(T) == 2 && DP <= 128) ? 2 : 1)
+    packed_mma_kernel(const PackedParams p) {
+  using Tile = MmaTile<T, DP>;
+  constexpr int kPieces = Tile::kPieces, kKeys = Tile::kKeys, kStep = Tile::kStep;
+  constexpr int kMine = kKeys / 2;  // keys of a tile that a warp takes
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(smem_raw);
+  __nv_bfloat16* ks = qs + kPieces * Tile::kQPiece;
+  __nv_bfloat16* vs = ks + kPieces * Tile::kKeyPiece;
 
   const int head = blockIdx.y, dim = p.dim;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Tiles with many keys first (causal): a long sequence's last rows would otherwise start last.
   const Piece piece = find_piece(p.batch, static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x, [&](int32_t b) {
     return (rows_of(p.offsets, b, p.rows_q, p.status).count + kTile - 1) / kTile;
@@ -90,9 +180,8 @@ __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_ke
   if (piece.sequence < 0) {
     const Rows rest = rows_behind(p.offsets, p.batch, p.rows_q);
     const int64_t first = piece.index * kTile;
-    for (int r = 0; r < kTile && first + r < rest.count; ++r)
-      for (int d = threadIdx.x; d < dim; d += kSimtThreads)
-        Elem<T>::store(out + ((rest.begin + first + r) * p.heads + head) * dim + d, 0.f);
+    for (int r = warp; r < kTile && first + r < rest.count; r += 8)
+      for (int d = lane; d < dim; d += 32) Elem<T>::store(out + ((rest.begin + first + r) * p.heads + head) * dim + d, 0.f);
     return;
   }
   const Rows mine = rows_of(p.offsets, piece.sequence, p.rows_q, nullptr);
@@ -107,154 +196,196 @@ __global__ void __launch_bounds__(kSimtThreads, DP <= 96 ? 2 : 1) packed_simt_ke
   const int kv_head = head / p.group;
   const T* k = static_cast<const T*>(p.k) + theirs.begin * p.k_row + kv_head * p.k_head;
   const T* v = static_cast<const T*>(p.v) + theirs.begin * p.v_row + kv_head * p.v_head;
+  mma_load<T, DP>(qs, Tile::kQPiece, q, p.q_row, kTile, rows, dim, p.vectors);
 
-  simt_load<T, DP>(qs, q, p.q_row, rows, dim, p.vectors);
-  if (keys > 0) simt_load<T, DP>(ks, k, p.k_row, static_cast<int>(keys < kTile ? keys : kTile), dim, p.vectors);
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float top[4], total[4], acc[4][kCols * 2];
+  const int run = warp & 3, half = warp >> 2, quad = lane & 3, octet = lane >> 2;
+  const uint32_t q_addr = smem_u32(qs + (run * 16 + (lane & 15)) * kStep + (lane >> 4) * 8);
+  const uint32_t k_addr = smem_u32(ks + (half * kMine + (lane & 7) + (lane >> 4) * 8) * kStep + ((lane >> 3) & 1) * 8);
+  const uint32_t v_addr = smem_u32(vs + (half * kMine + (lane & 15)) * kStep + (lane >> 4) * 8);
+  int64_t sees[2];  // keys that this thread's two rows see
+  float top[2], total[2], o[DP / 8][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    top[i] = -INFINITY;
-    total[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < kCols * 2; ++c) acc[i][c] = 0.f;
+  for (int e = 0; e < 2; ++e) {
+    const int64_t row = row0 + run * 16 + octet + 8 * e;
+    sees[e] = p.causal ? min(max(row + shift, int64_t{0}), theirs.count) : theirs.count;
+    top[e] = -INFINITY;
+    total[e] = 0.f;
   }
-  for (int64_t key0 = 0; key0 < keys; key0 += kTile) {
-    const int here = static_cast<int>(keys - key0 < kTile ? keys - key0 : kTile);
-    simt_loaded();  // K (and Q); V of the last tile has been read
-    simt_load<T, DP>(vs, v + key0 * p.v_row, p.v_row, here, dim, p.vectors);
-    float s[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+
+  for (int64_t key0 = 0; key0 < keys; key0 += kKeys) {
+    const int here = static_cast<int>(keys - key0 < kKeys ? keys - key0 : kKeys);
+    __syncthreads();  // the last tile has been read
+    mma_load<T, DP>(ks, Tile::kKeyPiece, k + key0 * p.k_row, p.k_row, kKeys, here, dim, p.vectors);
+    mma_load<T, DP>(vs, Tile::kKeyPiece, v + key0 * p.v_row, p.v_row, kKeys, here, dim, p.vectors);
+    __syncthreads();
+    float s[kMine / 8][4];
+#pragma unroll
+    for (int n = 0; n < kMine / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
 #pragma unroll 2
-    for (int d = 0; d < DP; d += 4) {
-      float4 a[4], b[4];
+    for (int d = 0; d < DP; d += 16) {
+      uint32_t a[kPieces][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * kStep + d);
+      for (int x = 0; x < kPieces; ++x) ldmatrix(a[x], q_addr + (x * Tile::kQPiece + d) * 2);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kStep + d);
+      for (int n = 0; n < kMine / 8; n += 2)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int y = 0; y < kPieces; ++y) {
+          uint32_t b[4];
+          ldmatrix(b, k_addr + (y * Tile::kKeyPiece + n * 8 * kStep + d) * 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
-    }
-    // Whether some row of the tile sees only a part of these keys.
-    const bool cut = p.causal && row0 + shift < key0 + here;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t limit = p.causal ? row0 + ty * 4 + i + shift - key0 : here;
-      float best = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = tx + 16 * j;
-        s[i][j] = key < here && key < limit ? s[i][j] * p.scale_log2 : -INFINITY;
-        best = fmaxf(best, s[i][j]);
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-      best = fmaxf(best, top[i]);
-      const float base = best == -INFINITY ? 0.f : best;  // nothing seen yet: every term is 2^-inf
-      const float keep = fast_exp2(top[i] - base);
-      top[i] = best;
-      total[i] *= keep;
-#pragma unroll
-      for (int c = 0; c < kCols * 2; ++c) acc[i][c] *= keep;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = fast_exp2(s[i][j] - base);
-        total[i] += s[i][j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4*>(ps + (tx + 16 * j) * kPStep + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
-    simt_loaded();  // V and P; K has been read
-    if (key0 + kTile < keys)
-      simt_load<T, DP>(ks, k + (key0 + kTile) * p.k_row, p.k_row, static_cast<int>(keys - key0 - kTile < kTile ? keys - key0 - kTile : kTile),
-                       dim, p.vectors);
-    // A masked value must not be read as 0 * value (it may be an infinity or NaN): where the mask cuts the tile, row i
-    // takes the keys below seen[i].
-    auto add_values = [&](auto masked) {
-      int seen[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) seen[i] = static_cast<int>(min(row0 + ty * 4 + i + shift - key0, int64_t{kTile}));
-#pragma unroll 4
-      for (int key = 0; key < here; ++key) {
-        const float4 a4 = *reinterpret_cast<const float4*>(ps + key * kPStep + ty * 4);
-        const float a[4] = {a4.x, a4.y, a4.z, a4.w};
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const float2 b = *reinterpret_cast<const float2*>(vs + key * kStep + c * 32 + tx * 2);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (decltype(masked)::value && key >= seen[i]) continue;
-            acc[i][c * 2] = fmaf(a[i], b.x, acc[i][c * 2]);
-            acc[i][c * 2 + 1] = fmaf(a[i], b.y, acc[i][c * 2 + 1]);
+          for (int x = 0; x + y < kPieces; ++x) {
+            mma_bf16(s[n], a[x], b[0], b[1]);
+            mma_bf16(s[n + 1], a[x], b[2], b[3]);
           }
         }
+    }
+    // Softmax of two rows, 2 * kMine / 8 keys each in this thread.
+    float best[2] = {-INFINITY, -INFINITY};
+    const int64_t first_key = key0 + half * kMine + 2 * quad;
+    const int seen[2] = {static_cast<int>(min(sees[0] - first_key, int64_t{kKeys})),
+                         static_cast<int>(min(sees[1] - first_key, int64_t{kKeys}))};
+#pragma unroll
+    for (int n = 0; n < kMine / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[n][i] = n * 8 + (i & 1) < seen[i >> 1] ? s[n][i] * p.scale_log2 : -INFINITY;
+        best[i >> 1] = fmaxf(best[i >> 1], s[n][i]);
       }
-    };
-    if (cut)
-      add_values(std::true_type{});
-    else
-      add_values(std::false_type{});
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      best[e] = fmaxf(best[e], __shfl_xor_sync(0xffffffffu, best[e], 1));
+      best[e] = fmaxf(fmaxf(best[e], __shfl_xor_sync(0xffffffffu, best[e], 2)), top[e]);
+      const float base = best[e] == -INFINITY ? 0.f : best[e];  // nothing seen yet: every term is 2^-inf
+      const float keep = fast_exp2(top[e] - base);
+      top[e] = best[e];
+      total[e] *= keep;
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) {
+        o[n][2 * e] *= keep;
+        o[n][2 * e + 1] *= keep;
+      }
+#pragma unroll
+      for (int n = 0; n < kMine / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[n][2 * e + i] = fast_exp2(s[n][2 * e + i] - base);
+          total[e] += s[n][2 * e + i];
+        }
+    }
+#pragma unroll
+    for (int key = 0; key < kMine; key += 16) {
+      uint32_t a[kPieces][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t pieces[kPieces];
+        to_pieces<kPieces>(s[key / 8 + i / 2][2 * (i & 1)], s[key / 8 + i / 2][2 * (i & 1) + 1], pieces);
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) a[x][i] = pieces[x];
+      }
+#pragma unroll
+      for (int n = 0; n < DP / 8; n += 2)
+#pragma unroll
+        for (int y = 0; y < kPieces; ++y) {
+          uint32_t b[4];
+          ldmatrix_trans(b, v_addr + (y * Tile::kKeyPiece + key * kStep + n * 8) * 2);
+#pragma unroll
+          for (int x = 0; x + y < kPieces; ++x) {
+            mma_bf16(o[n], a[x], b[0], b[1]);
+            mma_bf16(o[n + 1], a[x], b[2], b[3]);
+          }
+        }
+    }
   }
+  // The halves of the keys are joined: those of the second hand over maximum, sum and accumulator.
+  __syncthreads();
+  float* left = reinterpret_cast<float*>(smem_raw) + (run * 32 + lane) * (DP / 2 + 4);
+  if (half == 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+    for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float4*>(left + 4 * n) = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
+    *reinterpret_cast<float4*>(left + DP / 2) = make_float4(top[0], top[1], total[0], total[1]);
+  }
+  __syncthreads();
+  if (half == 1) return;
+  float mine_by[2], theirs_by[2];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) total[i] += __shfl_xor_sync(0xffffffffu, total[i], o);
-    const int r = ty * 4 + i;
-    if (r >= rows) continue;
-    const bool none = theirs.count == 0 || (p.causal && row0 + r + shift <= 0);
-    const float inv = none ? 0.f : 1.f / total[i];
-    T* dst = out + ((mine.begin + row0 + r) * p.heads + head) * dim;
+  for (int e = 0; e < 2; ++e) {
+    const float their_top = left[DP / 2 + e], best = fmaxf(top[e], their_top), base = best == -INFINITY ? 0.f : best;
+    const float a = fast_exp2(top[e] - base), b = fast_exp2(their_top - base);
+    float sum = total[e] * a + left[DP / 2 + 2 + e] * b;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    const float inv = sees[e] > 0 ? 1.f / sum : 0.f;
+    mine_by[e] = a * inv;
+    theirs_by[e] = b * inv;
+  }
+  bool fine[2] = {true, true};
 #pragma unroll
-    for (int c = 0; c < kCols; ++c)
+  for (int n = 0; n < DP / 8; ++n) {
+    const float4 more = *reinterpret_cast<const float4*>(left + 4 * n);
+    const float other[4] = {more.x, more.y, more.z, more.w};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int d = c * 32 + tx * 2 + j;
-        if (d < dim) Elem<T>::store(dst + d, none ? 0.f : acc[i][c * 2 + j] * inv);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int e = i >> 1, r = run * 16 + octet + 8 * e, d = n * 8 + 2 * quad + (i & 1);
+      const float value = sees[e] > 0 ? o[n][i] * mine_by[e] + other[i] * theirs_by[e] : 0.f;
+      fine[e] &= isfinite(value);
+      if (r < rows && d < dim) Elem<T>::store(out + ((mine.begin + row0 + r) * p.heads + head) * dim + d, value);
+    }
+  }
+  __syncwarp();  // a row's columns, which four threads have stored, may be stored again by another of them
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = run * 16 + octet + 8 * e;
+    const unsigned not_fine = __ballot_sync(0xffffffffu, !fine[e]);
+    if ((not_fine >> (lane & ~3) & 15u) == 0 || r >= rows) continue;
+    // Each of the four takes a quarter of the columns. f32: pieces turn every infinity into NaN, so the row is always taken again.
+    const int each = (dim + 3) / 4;
+    packed_row_again<T>(p, q + r * p.q_row, k, v, sees[e], keys, kPieces > 1, min(quad * each, dim), min((quad + 1) * each, dim),
+                        out + ((mine.begin + row0 + r) * p.heads + head) * dim);
   }
 }
 
-std::once_flag g_simt_attr_once[64];
+std::once_flag g_mma_attr_once[64];
 
 template <typename T, int DP>
-void launch_simt(const PackedParams& p, cudaStream_t s) {
+void launch_mma(const PackedParams& p, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(p.rows_q / kTile + p.batch + 1), static_cast<unsigned>(p.heads));
-  packed_simt_kernel<T, DP><<<grid, kSimtThreads, simt_smem_bytes<DP>(), s>>>(p);
+  packed_mma_kernel<T, DP><<<grid, kMmaThreads, MmaTile<T, DP>::kBytes, s>>>(p);
 }
-
 template <typename T, int DP>
-void simt_attribute() {
-  cudaFuncSetAttribute(packed_simt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       static_cast<int>(simt_smem_bytes<DP>()));
+void mma_attribute() {
+  cudaFuncSetAttribute(packed_mma_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       static_cast<int>(MmaTile<T, DP>::kBytes));
 }
 template <typename T>
-void simt_attributes() {
-  simt_attribute<T, 64>();
-  simt_attribute<T, 96>();
-  simt_attribute<T, 128>();
-  simt_attribute<T, 192>();
-  simt_attribute<T, 256>();
+void mma_attributes() {
+  mma_attribute<T, 64>();
+  mma_attribute<T, 80>();
+  mma_attribute<T, 96>();
+  mma_attribute<T, 128>();
+  mma_attribute<T, 192>();
+  mma_attribute<T, 256>();
 }
 
 template <typename T>
-void launch_simt_any(const PackedParams& p, cudaStream_t s) {
+void launch_mma_any(const PackedParams& p, cudaStream_t s) {
   if (p.dim <= 64)
-    launch_simt<T, 64>(p, s);
+    launch_mma<T, 64>(p, s);
+  else if (p.dim <= 80)
+    launch_mma<T, 80>(p, s);
   else if (p.dim <= 96)
-    launch_simt<T, 96>(p, s);
+    launch_mma<T, 96>(p, s);
   else if (p.dim <= 128)
-    launch_simt<T, 128>(p, s);
+    launch_mma<T, 128>(p, s);
   else if (p.dim <= 192)
-    launch_simt<T, 192>(p, s);
+    launch_mma<T, 192>(p, s);
   else
-    launch_simt<T, 256>(p, s);
+    launch_mma<T, 256>(p, s);
 }
 
 // ------------------------------------------------------------------------- bf16, head size 64 or 128
@@ -280,9 +411,7 @@ void launch_simt_any(const PackedParams& p, cudaStream_t s) {
 // of 80 keys, which ends the waiting but costs more softmax and MMA time a key (519 against 482 us); 16 softmax warps, two to a
 // row (496); taking turns at the exponentials (506); the maximum taken alongside stale exponentials (519); a cubic
 // for 0, 1/4 or 3/8 of the exponentials in place of 1/8 (491, 482, 530 against 468).
-// Masks cost only the blocks that they cut. A value that a row does not see still meets P = 0 in the product, and
-// 0 * infinity would be NaN: a row whose result is not finite looks whether such a value lay in the blocks that its mask cuts, and
-// is computed again without the tensor core if so.
+// Masks cost only the blocks that they cut.
 constexpr int kQRows = 128, kKeys = 128;
 constexpr int kUmmaThreads = 384, kUmmaProducerWarp = 8, kUmmaMmaWarp = 9;
 constexpr uint32_t kUmmaScoreCols = 128, kUmmaOutCol = 256;
@@ -315,47 +444,6 @@ struct UmmaParams {
   int32_t head_pairs;  // 1: the two tiles are two heads; 0: two runs of rows
   uint32_t idesc_qk, idesc_pv;
 };
-
-// One row again, by one thread: what the tensor core cannot do without touching unseen values.
-template <int D>
-__device__ __forceinline__ void packed_row_again(const PackedParams& p, const __nv_bfloat16* q, const __nv_bfloat16* k,
-                                              const __nv_bfloat16* v, int64_t sees, int64_t read, __nv_bfloat16* dst) {
-  bool touched = false;
-  for (int64_t j = sees; j < read && !touched; ++j)
-    for (int d = 0; d < D; d += 8) {
-      const uint4 w = ld_plain16(v + j * p.v_row + d);
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        touched |= (words[i] & 0x7f80u) == 0x7f80u || (words[i] & 0x7f800000u) == 0x7f800000u;
-    }
-  if (!touched) return;  // the row itself is not finite
-  float acc[D], top = -INFINITY, total = 0.f;
-  for (int d = 0; d < D; ++d) acc[d] = 0.f;
-  for (int64_t j = 0; j < sees; ++j) {
-    float s = 0.f;
-    for (int d = 0; d < D; d += 8) {
-      float a[8], b[8];
-      unpack16(ld_plain16(q + d), a);
-      unpack16(ld_plain16(k + j * p.k_row + d), b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
-    }
-    s *= p.scale_log2;
-    const float best = fmaxf(top, s), base = best == -INFINITY ? 0.f : best;
-    const float keep = fast_exp2(top - base), weight = fast_exp2(s - base);
-    top = best;
-    total = fmaf(total, keep, weight);
-    for (int d = 0; d < D; d += 8) {
-      float b[8];
-      unpack16(ld_plain16(v + j * p.v_row + d), b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[d + i] = fmaf(weight, b[i], acc[d + i] * keep);
-    }
-  }
-  const float inv = 1.f / total;
-  for (int d = 0; d < D; ++d) dst[d] = __float2bfloat16_rn(acc[d] * inv);
-}
 
 // 2^x for two values on the FMA pipe, |relative error| < 8.6e-5 (P is rounded to 2^-9): x = n + r with n the whole number below
 // (adding 1.5 * 2^23 rounded down), a cubic for 2^r over [0, 1) that is 1 at 0 and was fitted for the least
@@ -703,7 +791,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k) + theirs.begin * p.k_row + kv_head * p.k_head;
         const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v) + theirs.begin * p.v_row + kv_head * p.v_head;
         const int64_t read = min(static_cast<int64_t>(my_blocks) * kKeys, p.rows_k - theirs.begin);
-        packed_row_again<D>(p, q, k, v, sees, read, dst);
+        packed_row_again<__nv_bfloat16>(p, q, k, v, sees, read, false, 0, D, dst);
       }
     }
   }
@@ -811,9 +899,9 @@ extern "C" int b200_attention_packed(const b200_packed_attention_desc* desc, voi
   p.scale_log2 = d.scale * kLog2e;
   p.status = kernel_status_word();
 
-  std::call_once(g_simt_attr_once[dev.device], [] {
-    simt_attributes<float>();
-    simt_attributes<__nv_bfloat16>();
+  std::call_once(g_mma_attr_once[dev.device], [] {
+    mma_attributes<float>();
+    mma_attributes<__nv_bfloat16>();
   });
   std::call_once(g_umma_attr_once[dev.device], [] {
     cudaFuncSetAttribute(packed_umma_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -823,8 +911,8 @@ extern "C" int b200_attention_packed(const b200_packed_attention_desc* desc, voi
   });
   if (umma_takes(d)) return d.dim == 64 ? launch_umma<64>(p, d, s) : launch_umma<128>(p, d, s);
   if (d.dtype == B200_F32)
-    launch_simt_any<float>(p, s);
+    launch_mma_any<float>(p, s);
   else
-    launch_simt_any<__nv_bfloat16>(p, s);
+    launch_mma_any<__nv_bfloat16>(p, s);
   return launched();
 }

@@ -19,13 +19,13 @@ constexpr uint32_t kInfBits = 0x7f800000u;
 // of both kernels otherwise (a write of prompts 55 us in place of 20).
 constexpr float kWhole = 12582912.f;
 // x / s to the nearest, as the bits of kWhole + code (the low byte is the code): `inv` is within 2^-23 of 1 / s, so the result can
-// only be wrong next to a tie, which `near_tie` tells from the remainder.
-__device__ __forceinline__ float quotient(float x, float s, float inv, bool& near_tie) {
+// only be wrong next to a tie, where the remainder is near s / 2 (`rest` keeps the largest).
+__device__ __forceinline__ float quotient(float x, float s, float inv, float& rest) {
   const float shifted = fmaf(x, inv, kWhole);
-  const float rest = fmaf(-(shifted - kWhole), s, x);
-  near_tie |= fabsf(rest) > 0.4999f * s;
+  rest = fmaxf(rest, fabsf(fmaf(kWhole - shifted, s, x)));
   return shifted;
 }
+constexpr float kNearTie = 0.4999f;
 // rint(x / s), ties to even: the guess moved by the exact signs of x - (r +- 1/2) s (one rounding of an exact product and
 // sum: the sign is right, and zero is a tie).
 __device__ __forceinline__ float quotient_at_tie(float x, float s, float shifted) {
@@ -225,24 +225,32 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
       }
     }
   }
-  if (any_new) {
+  if (!finite) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (is_new(j))
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t& w = word[is_v ? i : 2 * j + i / 4];
+          w = with_code(w, is_v ? j : i & 3, kWhole);
+        }
+  } else if (any_new) {
     const float inv = __frcp_rn(s);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (!is_new(j)) continue;
-      float x[8], code[8];
+      float x[8], code[8], rest = 0.f;
       here[j].values(x);
-      bool near_tie = false;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) code[i] = quotient(x[i], s, inv, near_tie);
-      if (near_tie) {
+      for (int i = 0; i < 8; ++i) code[i] = quotient(x[i], s, inv, rest);
+      if (rest > kNearTie * s) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) code[i] = quotient_at_tie(x[i], s, code[i]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint32_t& w = word[is_v ? i : 2 * j + i / 4];
-        w = with_code(w, is_v ? j : i & 3, finite ? code[i] : kWhole);
+        w = with_code(w, is_v ? j : i & 3, code[i]);
       }
     }
   }
@@ -348,11 +356,10 @@ __global__ void __launch_bounds__(256) kv_append_few_kernel(const AppendParams p
   const float inv = __frcp_rn(s);
   for (int slot = first; slot < stop; ++slot) {
     if (slot > first) load_channels<T, PER>(src + slot * step, x);
-    bool near_tie = false;
-    float code[PER];
+    float code[PER], rest = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) code[i] = quotient(x[i], s, inv, near_tie);
-    if (near_tie) {
+    for (int i = 0; i < PER; ++i) code[i] = quotient(x[i], s, inv, rest);
+    if (rest > kNearTie * s) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) code[i] = quotient_at_tie(x[i], s, code[i]);
     }

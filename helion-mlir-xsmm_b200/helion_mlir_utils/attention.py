@@ -123,7 +123,7 @@ def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: T
 
 
 def _tensor_core(q: Tensor, scale: float) -> bool:
-    """Whether the tcgen05 kernel takes these operands (else f32 tiles on the CUDA cores)."""
+    """Whether the tcgen05 kernel takes these operands (else mma tiles of any head size)."""
     return q.dtype is torch.bfloat16 and q.shape[2] in _FUSED_DIMS and scale > 0.0
 
 
@@ -174,7 +174,7 @@ def _explain_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets:
     _check_packed(q, k, v, offsets, offsets if k_offsets is None else k_offsets)
     if _tensor_core(q, 1.0 if scale is None else scale):
         return CallExplanation(True, "packed_umma_kernel (tcgen05, two tiles of 128 queries x 128 keys per step, scores in TMEM)")
-    return CallExplanation(True, "packed_simt_kernel (f32 tiles of 64 x 64)")
+    return CallExplanation(True, "packed_mma_kernel (mma bf16, f32 values in three pieces, 64 queries a CTA)")
 
 
 attention_packed.explain = _explain_packed  # type: ignore[attr-defined]
