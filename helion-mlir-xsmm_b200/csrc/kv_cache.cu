@@ -54,13 +54,18 @@ __device__ __forceinline__ uint32_t with_code(uint32_t word, int i, float code) 
   return __byte_perm(word, __float_as_uint(code), i == 0 ? 0x3214 : (i == 1 ? 0x3240 : (i == 2 ? 0x3410 : 0x4210)));
 }
 
-// 8 consecutive values as they lie in memory.
+// A thread's eight channels of a token: 16 bytes next to each other for bf16, and for f32 16 bytes in either half of the head, so
+// that neighbouring threads always touch neighbouring 16 bytes. channel_of is the i-th.
+template <typename T>
+__device__ __forceinline__ int channel_of(int part, int i, int dim) {
+  return sizeof(T) == 2 ? part * 8 + i : (i >> 2) * (dim >> 1) + part * 4 + (i & 3);
+}
 template <typename T>
 struct Eight {
   uint4 raw[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
+  __device__ __forceinline__ void load(const T* token, int part, int dim) {
 #pragma unroll
-    for (unsigned i = 0; i < sizeof(T) / 2; ++i) raw[i] = ld_stream16(p + i * Elem<T>::kVec);
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) raw[i] = ld_stream16(token + channel_of<T>(part, i * Elem<T>::kVec, dim));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -92,12 +97,38 @@ struct Eight {
     }
   }
 };
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+__device__ __forceinline__ void store8(float* token, int part, int dim, const float (&v)[8]) {
   const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-  st_stream16(p, pack16(a));
-  st_stream16(p + 4, pack16(b));
+  st_stream16(token + channel_of<float>(part, 0, dim), pack16(a));
+  st_stream16(token + channel_of<float>(part, 4, dim), pack16(b));
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) { st_stream16(p, pack16(v)); }
+__device__ __forceinline__ void store8(__nv_bfloat16* token, int part, int dim, const float (&v)[8]) {
+  st_stream16(token + part * 8, pack16(v));
+}
+// Those channels' codes of a token of K: two words.
+template <typename T>
+__device__ __forceinline__ uint2 load_codes(const int8_t* token, int part, int dim) {
+  if (sizeof(T) == 2) return *reinterpret_cast<const uint2*>(token + part * 8);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(token + channel_of<T>(part, 0, dim)),
+                    *reinterpret_cast<const uint32_t*>(token + channel_of<T>(part, 4, dim)));
+}
+template <typename T>
+__device__ __forceinline__ void store_codes(int8_t* token, int part, int dim, uint32_t lo, uint32_t hi) {
+  if (sizeof(T) == 2) {
+    *reinterpret_cast<uint2*>(token + part * 8) = make_uint2(lo, hi);
+  } else {
+    *reinterpret_cast<uint32_t*>(token + channel_of<T>(part, 0, dim)) = lo;
+    *reinterpret_cast<uint32_t*>(token + channel_of<T>(part, 4, dim)) = hi;
+  }
+}
+// A block of V in shared memory, as words of four tokens: word g of channel r. Every run of channels that one thread holds starts
+// a bank further on, so that neighbouring threads' words do not collide.
+constexpr int kTurnWords = 64 / 4 * 128 + 128 / 4;
+template <typename T>
+__device__ __forceinline__ int turn_at(int r, int g, int groups) {
+  constexpr int kRun = Elem<T>::kVec;
+  return r / kRun * (kRun * groups + 1) + r % kRun * groups + g;
+}
 
 struct AppendParams {
   Cache cache;
@@ -146,22 +177,22 @@ __device__ __forceinline__ float new_scale(uint32_t largest, float before, bool&
   return finite ? s : __uint_as_float(0x7fc00000u);
 }
 
-// A thread holds 8 values of each of 4 consecutive tokens. Threads of a warp go along the head first
-// for K (8 code bytes of a token next to each other) and along the tokens first for V (4 codes of a
-// channel in one word, the words of a channel next to each other), so both leave in whole sectors. A CTA is one chain of
+// A thread holds 8 values of each of 4 consecutive tokens; the threads of a warp go along the head first, so values are read
+// and K's codes written in whole lines. V's codes lie the other way round: a block that is written whole is turned
+// in shared memory (words of four tokens) and leaves as one run of lines; of one that is not, each thread
+// writes its words. A CTA is one chain of
 // dependent loads (lengths, then its values and the table, then the block's scale and codes): what counts is how many
 // are on an SM, so registers are held to four CTAs of 256 threads.
 template <typename T, bool is_v>
-__device__ __forceinline__ void append_block(const AppendParams& p) {
+__device__ __forceinline__ void append_block(const AppendParams& p, uint32_t* turn) {
   const Cache& c = p.cache;
   AppendPlace place;
   if (!find_append(p, place)) return;
   const int first = place.first, stop = place.stop;
   const int head = blockIdx.y, parts = c.dim / 8, groups = c.tokens / 4;
-  const int part = is_v ? threadIdx.x / groups : threadIdx.x % parts;
-  const int slot0 = 4 * (is_v ? threadIdx.x % groups : threadIdx.x / parts);
+  const int part = threadIdx.x % parts, slot0 = threadIdx.x / parts * 4;
   const int64_t step = is_v ? p.v_row : p.k_row;
-  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + part * 8 + place.row * step + head * (is_v ? p.v_head : p.k_head);
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + place.row * step + head * (is_v ? p.v_head : p.k_head);
   auto is_new = [&](int j) { return slot0 + j >= first && slot0 + j < stop; };
   const bool any_new = slot0 + 4 > first && slot0 < stop, all_new = slot0 >= first && slot0 + 4 <= stop;
   const bool any_old = slot0 < first;
@@ -170,7 +201,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (is_new(j))
-      here[j].load(src + (slot0 + j) * step);
+      here[j].load(src + (slot0 + j) * step, part, c.dim);
     else
       here[j].clear();
   }
@@ -187,11 +218,12 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
   if (is_v ? (any_old || any_new) && !all_new : any_old) {
     if (is_v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) word[i] = *reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0);
+      for (int i = 0; i < 8; ++i)
+        word[i] = *reinterpret_cast<const uint32_t*>(codes + channel_of<T>(part, i, c.dim) * c.tokens + slot0);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint2 w = *reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8);
+        const uint2 w = load_codes<T>(codes + (slot0 + j) * c.dim, part, c.dim);
         word[2 * j] = w.x;
         word[2 * j + 1] = w.y;
       }
@@ -254,25 +286,39 @@ __device__ __forceinline__ void append_block(const AppendParams& p) {
       }
     }
   }
-  if (is_v) {
-    if (any_new || (grew && any_old)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0) = word[i];
-    }
-  } else {
+  if (!is_v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (is_new(j) || (grew && slot0 + j < first))
-        *reinterpret_cast<uint2*>(codes + (slot0 + j) * c.dim + part * 8) = make_uint2(word[2 * j], word[2 * j + 1]);
+        store_codes<T>(codes + (slot0 + j) * c.dim, part, c.dim, word[2 * j], word[2 * j + 1]);
+  } else if (first == 0 && stop == c.tokens) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turn[turn_at<T>(channel_of<T>(part, i, c.dim), slot0 / 4, groups)] = word[i];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int at = 4 * (threadIdx.x + n * blockDim.x), r = at / groups, g = at % groups;
+      uint4 w;
+      w.x = turn[turn_at<T>(r, g, groups)];
+      w.y = turn[turn_at<T>(r, g + 1, groups)];
+      w.z = turn[turn_at<T>(r, g + 2, groups)];
+      w.w = turn[turn_at<T>(r, g + 3, groups)];
+      *reinterpret_cast<uint4*>(codes + 4 * at) = w;
+    }
+  } else if (any_new || (grew && any_old)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<uint32_t*>(codes + channel_of<T>(part, i, c.dim) * c.tokens + slot0) = word[i];
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) kv_append_kernel(const AppendParams p) {
+  __shared__ uint32_t turn[kTurnWords];
   if (blockIdx.z)
-    append_block<T, true>(p);
+    append_block<T, true>(p, turn);
   else
-    append_block<T, false>(p);
+    append_block<T, false>(p, turn);
 }
 
 // The same write when the blocks get few tokens each (single tokens of many sequences): a warp for each (block, head,
@@ -393,13 +439,12 @@ struct ReadParams {
 
 // The same division of a block among threads as in the write, the other way round.
 template <typename T, bool is_v>
-__device__ __forceinline__ void read_block(const ReadParams& p) {
+__device__ __forceinline__ void read_block(const ReadParams& p, uint32_t* turn) {
   const Cache& c = p.cache;
   const int parts = c.dim / 8, groups = c.tokens / 4;
-  const int part = is_v ? threadIdx.x / groups : threadIdx.x % parts;
-  const int slot0 = 4 * (is_v ? threadIdx.x % groups : threadIdx.x / parts);
+  const int part = threadIdx.x % parts, slot0 = threadIdx.x / parts * 4;
   const int head0 = blockIdx.y * p.heads_each, head_end = min(head0 + p.heads_each, c.heads);
-  T* out = static_cast<T*>(is_v ? p.v_out : p.k_out) + part * 8;
+  T* out = static_cast<T*>(is_v ? p.v_out : p.k_out);
   const int64_t step = static_cast<int64_t>(c.heads) * c.dim;
   const Piece piece = find_piece(p.batch, blockIdx.x, [&](int32_t b) {
     const int64_t n = rows_of(p.offsets, b, p.rows, p.status).count, start = max(p.starts[b], 0);
@@ -412,7 +457,7 @@ __device__ __forceinline__ void read_block(const ReadParams& p) {
     for (int j = 0; j < 4; ++j) {
       const int64_t r = (piece.index << c.token_bits) + slot0 + j;
       if (r < rest.count)
-        for (int head = head0; head < head_end; ++head) store8(out + (rest.begin + r) * step + head * c.dim, none);
+        for (int head = head0; head < head_end; ++head) store8(out + (rest.begin + r) * step + head * c.dim, part, c.dim, none);
     }
     return;
   }
@@ -425,24 +470,29 @@ __device__ __forceinline__ void read_block(const ReadParams& p) {
   out += (rows.begin + start - from) * step;
   int64_t block = -1;
   if (held > first) block = block_of(c, p.table, piece.sequence, page, p.status);
-  const bool any = slot0 + 4 > first && slot0 < held && block >= 0;
+  const bool any = slot0 + 4 > first && slot0 < held;
 
-  uint32_t next[8];
+  uint32_t next[8];  // K: two words of each token; V: eight words of the block as it lies, to be turned
   float next_scale = held > first ? __uint_as_float(0x7fc00000u) : 0.f;  // (a bad block)
 #pragma unroll
   for (int i = 0; i < 8; ++i) next[i] = 0;
   auto fetch = [&](int head) {
-    if (!any) return;
+    if (block < 0) return;
     next_scale = (is_v ? c.v_scales : c.k_scales)[block * c.heads + head];
     const int8_t* codes = (is_v ? c.v_codes : c.k_codes) + (block * c.heads + head) * c.tokens * c.dim;
     if (is_v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        next[i] = __ldg(reinterpret_cast<const uint32_t*>(codes + (part * 8 + i) * c.tokens + slot0));
-    } else {
+      for (int n = 0; n < 2; ++n) {
+        const uint4 w = ld_stream16(codes + 16 * (threadIdx.x + n * blockDim.x));
+        next[4 * n] = w.x;
+        next[4 * n + 1] = w.y;
+        next[4 * n + 2] = w.z;
+        next[4 * n + 3] = w.w;
+      }
+    } else if (any) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + (slot0 + j) * c.dim + part * 8));
+        const uint2 w = load_codes<T>(codes + (slot0 + j) * c.dim, part, c.dim);
         next[2 * j] = w.x;
         next[2 * j + 1] = w.y;
       }
@@ -451,8 +501,20 @@ __device__ __forceinline__ void read_block(const ReadParams& p) {
   fetch(head0);
   for (int head = head0; head < head_end; ++head) {
     uint32_t word[8];
+    if (is_v) {
+      if (head > head0) __syncthreads();  // the last head's words have been taken
 #pragma unroll
-    for (int i = 0; i < 8; ++i) word[i] = next[i];
+      for (int i = 0; i < 8; ++i) {
+        const int at = 4 * (threadIdx.x + (i >> 2) * blockDim.x) + (i & 3);
+        turn[turn_at<T>(at / groups, at % groups, groups)] = next[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) word[i] = turn[turn_at<T>(channel_of<T>(part, i, c.dim), slot0 / 4, groups)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) word[i] = next[i];
+    }
     const float s = next_scale;
     if (head + 1 < head_end) fetch(head + 1);
 #pragma unroll
@@ -464,17 +526,18 @@ __device__ __forceinline__ void read_block(const ReadParams& p) {
         const float code = is_v ? code_value(word[i], j) : code_value(word[2 * j + i / 4], i & 3);
         x[i] = slot0 + j < held ? code * s : 0.f;
       }
-      store8(out + (slot0 + j) * step + head * c.dim, x);
+      store8(out + (slot0 + j) * step + head * c.dim, part, c.dim, x);
     }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
+  __shared__ uint32_t turn[kTurnWords];
   if (blockIdx.z)
-    read_block<T, true>(p);
+    read_block<T, true>(p, turn);
   else
-    read_block<T, false>(p);
+    read_block<T, false>(p, turn);
 }
 
 // Heads for one CTA: as many as leave twelve CTAs to an SM (a power of two, so that little is left over).
