@@ -21,6 +21,8 @@ prefix back for ``attention_packed`` of a later chunk of the prompt.
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -182,6 +184,14 @@ def _check_cached(q: Tensor, heads: int, dim: int, batch: int) -> tuple[int, int
     return code, 1 if rank == 3 else q.shape[1], q.shape[-2]
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(index: int, heads: int, dim: int, block_tokens: int, width: int, batch: int, tokens: int, q_heads: int) -> int:
+    """Scratch of a call on device ``index``, which goes by sizes alone."""
+    desc = native.CachedAttentionDesc(cache=native.KvCacheDesc(heads=heads, dim=dim, block_tokens=block_tokens), table_width=width,
+                                      batch=batch, tokens=tokens, heads=q_heads)
+    return native.module().b200_attention_cached_workspace_bytes(ctypes.byref(desc))
+
+
 def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor, lengths: Tensor,
                      scale: float | None = None) -> Tensor:
     """``softmax(scale * q @ k^T) @ v`` over the cached positions; ``scale`` defaults to ``dim ** -0.5``.
@@ -196,20 +206,17 @@ def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], bl
     code, tokens, heads = _check_cached(q, fields[5], dim, batch)
     lengths_ptr = _indices("attention_cached", "lengths", lengths, batch)
     index = native.index_of(q, *cache, block_table, lengths)
-    lib = native.module()
     with native.on_index(index):
         if q.stride(-1) != 1:
             q = q.contiguous()
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-
-        def desc(workspace: int, held: int) -> bytes:
-            return _PACK_CACHED(*fields, code, 1.0 / math.sqrt(dim) if scale is None else scale, q.data_ptr(), out.data_ptr(),
-                                q.stride(0), q.stride(1) if tokens > 1 else 0, q.stride(-2), block_table.data_ptr(), lengths_ptr,
-                                stride, width, batch, tokens, heads, workspace, held)
-
-        need = lib.b200_attention_cached_workspace_bytes(desc(0, 0))
+        need = _workspace_bytes(index, fields[5], dim, fields[7], width, batch, tokens, heads)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        result = lib.b200_attention_cached(desc(workspace.data_ptr(), need), native.raw_stream(index))
+        result = native.module().b200_attention_cached(
+            _PACK_CACHED(*fields, code, 1.0 / math.sqrt(dim) if scale is None else scale, q.data_ptr(), out.data_ptr(), q.stride(0),
+                         q.stride(1) if tokens > 1 else 0, q.stride(-2), block_table.data_ptr(), lengths_ptr, stride, width, batch,
+                         tokens, heads, workspace.data_ptr(), need),
+            native.raw_stream(index))
     native.check("b200_attention_cached", result)
     return out
 
