@@ -70,8 +70,8 @@ __device__ __forceinline__ void packed_row_again(const PackedParams& p, const T*
 
 // One CTA takes 64 query rows of one head and goes over the keys in tiles, with the running maximum and sum of the
 // softmax in f32. Eight warps: four runs of 16 rows, two halves of each tile's keys, joined at the end. The products are
-// mma m16n8k16 on bf16 pieces: an f32 value is the sum of three (8 + 8 + 8 bits, the exponent range of f32, so nothing
-// has to be scaled), and a product the six of their products that reach 2^-24; Q, K, V and P alike. That is f32's own
+// mma m16n8k16 on bf16 pieces: an f32 value is the sum of three (8 bits each, the exponent range of f32, so nothing
+// has to be scaled), and a product the six of their products that reach 2^-27; Q, K, V and P alike. That is f32's own
 // accuracy at six instructions; FFMA tiles of 64 x 64 stood still on shared memory at a third of FFMA's rate (five
 // sequences of 300, 6 heads of 80: 84 us; one of 4096, 8 heads of 64: 775 us). bf16 values are one piece.
 constexpr int kTile = 64, kMmaThreads = 256;
@@ -105,20 +105,18 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two values as bf16 pairs: one, rounded to the nearest, or three, each the upper 16 bits of what the ones before leave over
-// (cut off, not rounded: nothing overflows, and the last takes the rest exactly).
+// Two values as PIECES bf16 pairs, each what the ones before leave over, rounded to the nearest: the second is at most 2^-9 of the
+// value, the third 2^-18 (of either sign: the products that are left out do not add up). An infinity, or a value that rounds to one,
+// leaves NaN over.
 template <int PIECES>
 __device__ __forceinline__ void to_pieces(float lo, float hi, uint32_t (&piece)[PIECES]) {
-  if (PIECES == 1) {
-    piece[0] = pack_bf16x2(lo, hi);
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const uint32_t a = __float_as_uint(lo), b = __float_as_uint(hi);
-    piece[i] = __byte_perm(a, b, 0x7632);
-    lo -= __uint_as_float(a & 0xffff0000u);
-    hi -= __uint_as_float(b & 0xffff0000u);
+    piece[i] = pack_bf16x2(lo, hi);
+    if (i + 1 < PIECES) {
+      lo -= __uint_as_float(piece[i] << 16);
+      hi -= __uint_as_float(piece[i] & 0xffff0000u);
+    }
   }
 }
 
@@ -165,6 +163,7 @@ __global__ void __launch_bounds__(kMmaThreads, DP <= 96 || (sizeof(T) == 2 && DP
   using Tile = MmaTile<T, DP>;
   constexpr int kPieces = Tile::kPieces, kKeys = Tile::kKeys, kStep = Tile::kStep;
   constexpr int kMine = kKeys / 2;  // keys of a tile that a warp takes
+  constexpr int kRun = kPieces > 1 ? 32 : DP;  // channels between two additions to the scores
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(smem_raw);
   __nv_bfloat16* ks = qs + kPieces * Tile::kQPiece;
@@ -227,26 +226,41 @@ __global__ void __launch_bounds__(kMmaThreads, DP <= 96 || (sizeof(T) == 2 && DP
     for (int n = 0; n < kMine / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-#pragma unroll 2
-    for (int d = 0; d < DP; d += 16) {
-      uint32_t a[kPieces][4];
+    // The tensor core cuts its sums off where f32 rounds them, always towards zero: f32 products of pieces go into fresh
+    // accumulators every 32 channels, the leading one apart from the others, and are added up by the FMA pipe.
+#pragma unroll 1
+    for (int d0 = 0; d0 < DP; d0 += kRun) {
+      float lead[kMine / 8][4], rest[kMine / 8][4];
 #pragma unroll
-      for (int x = 0; x < kPieces; ++x) ldmatrix(a[x], q_addr + (x * Tile::kQPiece + d) * 2);
+      for (int n = 0; n < kMine / 8; ++n)
 #pragma unroll
-      for (int n = 0; n < kMine / 8; n += 2)
+        for (int i = 0; i < 4; ++i) lead[n][i] = rest[n][i] = 0.f;
 #pragma unroll
-        for (int y = 0; y < kPieces; ++y) {
-          uint32_t b[4];
-          ldmatrix(b, k_addr + (y * Tile::kKeyPiece + n * 8 * kStep + d) * 2);
+      for (int d = d0; d < d0 + kRun; d += 16) {
+        if (DP % kRun && d >= DP) break;
+        uint32_t a[kPieces][4];
 #pragma unroll
-          for (int x = 0; x + y < kPieces; ++x) {
-            mma_bf16(s[n], a[x], b[0], b[1]);
-            mma_bf16(s[n + 1], a[x], b[2], b[3]);
+        for (int x = 0; x < kPieces; ++x) ldmatrix(a[x], q_addr + (x * Tile::kQPiece + d) * 2);
+#pragma unroll
+        for (int n = 0; n < kMine / 8; n += 2)
+#pragma unroll
+          for (int y = 0; y < kPieces; ++y) {
+            uint32_t b[4];
+            ldmatrix(b, k_addr + (y * Tile::kKeyPiece + n * 8 * kStep + d) * 2);
+#pragma unroll
+            for (int x = 0; x + y < kPieces; ++x) {
+              mma_bf16(x + y ? rest[n] : lead[n], a[x], b[0], b[1]);
+              mma_bf16(x + y ? rest[n + 1] : lead[n + 1], a[x], b[2], b[3]);
+            }
           }
-        }
+      }
+#pragma unroll
+      for (int n = 0; n < kMine / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] += kPieces > 1 ? lead[n][i] + rest[n][i] : lead[n][i];
     }
     // Softmax of two rows, 2 * kMine / 8 keys each in this thread.
-    float best[2] = {-INFINITY, -INFINITY};
+    float best[2] = {-INFINITY, -INFINITY}, kept[2];
     const int64_t first_key = key0 + half * kMine + 2 * quad;
     const int seen[2] = {static_cast<int>(min(sees[0] - first_key, int64_t{kKeys})),
                          static_cast<int>(min(sees[1] - first_key, int64_t{kKeys}))};
@@ -265,11 +279,7 @@ __global__ void __launch_bounds__(kMmaThreads, DP <= 96 || (sizeof(T) == 2 && DP
       const float keep = fast_exp2(top[e] - base);
       top[e] = best[e];
       total[e] *= keep;
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        o[n][2 * e] *= keep;
-        o[n][2 * e + 1] *= keep;
-      }
+      kept[e] = keep;
 #pragma unroll
       for (int n = 0; n < kMine / 8; ++n)
 #pragma unroll
@@ -278,28 +288,36 @@ __global__ void __launch_bounds__(kMmaThreads, DP <= 96 || (sizeof(T) == 2 && DP
           total[e] += s[n][2 * e + i];
         }
     }
+    uint32_t a[kMine / 16][kPieces][4];
 #pragma unroll
-    for (int key = 0; key < kMine; key += 16) {
-      uint32_t a[kPieces][4];
+    for (int key = 0; key < kMine; key += 16)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t pieces[kPieces];
         to_pieces<kPieces>(s[key / 8 + i / 2][2 * (i & 1)], s[key / 8 + i / 2][2 * (i & 1) + 1], pieces);
 #pragma unroll
-        for (int x = 0; x < kPieces; ++x) a[x][i] = pieces[x];
+        for (int x = 0; x < kPieces; ++x) a[key / 16][x][i] = pieces[x];
       }
 #pragma unroll
-      for (int n = 0; n < DP / 8; n += 2)
+    for (int n = 0; n < DP / 8; n += 2) {
+      float lead[2][4] = {}, rest[2][4] = {};  // of this tile
+#pragma unroll
+      for (int key = 0; key < kMine; key += 16)
 #pragma unroll
         for (int y = 0; y < kPieces; ++y) {
           uint32_t b[4];
           ldmatrix_trans(b, v_addr + (y * Tile::kKeyPiece + key * kStep + n * 8) * 2);
 #pragma unroll
           for (int x = 0; x + y < kPieces; ++x) {
-            mma_bf16(o[n], a[x], b[0], b[1]);
-            mma_bf16(o[n + 1], a[x], b[2], b[3]);
+            mma_bf16(x + y ? rest[0] : lead[0], a[key / 16][x], b[0], b[1]);
+            mma_bf16(x + y ? rest[1] : lead[1], a[key / 16][x], b[2], b[3]);
           }
         }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[n + m][i] = fmaf(o[n + m][i], kept[i >> 1], kPieces > 1 ? lead[m][i] + rest[m][i] : lead[m][i]);
     }
   }
   // The halves of the keys are joined: those of the second hand over maximum, sum and accumulator.
@@ -343,7 +361,7 @@ __global__ void __launch_bounds__(kMmaThreads, DP <= 96 || (sizeof(T) == 2 && DP
     const int r = run * 16 + octet + 8 * e;
     const unsigned not_fine = __ballot_sync(0xffffffffu, !fine[e]);
     if ((not_fine >> (lane & ~3) & 15u) == 0 || r >= rows) continue;
-    // Each of the four takes a quarter of the columns. f32: pieces turn every infinity into NaN, so the row is always taken again.
+    // Each of the four takes a quarter of the columns. f32: pieces turn infinities into NaN, so the row is always taken again.
     const int each = (dim + 3) / 4;
     packed_row_again<T>(p, q + r * p.q_row, k, v, sees[e], keys, kPieces > 1, min(quad * each, dim), min((quad + 1) * each, dim),
                         out + ((mine.begin + row0 + r) * p.heads + head) * dim);
