@@ -23,7 +23,8 @@
 //   * P carries V's scale: with t = score + log2(v_scale), P = 2^(t - max t) is at most 1 for every row,
 //     whatever the sizes of the blocks' values. It is rounded to f16 (2^-11; from 2^10 down to 2^-24, so
 //     nothing within 2^-34 of the row's largest is lost); the denominator is summed in f32 before that.
-//   * f32 queries: Q and P as the sum of two f16 values each, two products in place of one.
+//   * f32 queries: Q and P as the sum of two f16 values each, two products in place of one, into fresh accumulators every 64
+//     channels and every tile: the tensor core cuts its sums off, always towards zero, where f32 rounds them.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -363,6 +364,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::kWarps, 1) cached_kernel(const C
           const uint4 first = *reinterpret_cast<const uint4*>(tile + 4 * m * D + half * 64);
           const uint4 second = *reinterpret_cast<const uint4*>(tile + (4 * m + 2) * D + half * 64);
           const uint32_t w0[4] = {first.x, first.y, first.z, first.w}, w1[4] = {second.x, second.y, second.z, second.w};
+          float fresh[kSplit ? 2 : 1][NT][4] = {};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t a[4];
@@ -370,9 +372,15 @@ __global__ void __launch_bounds__(32 * Ring<D>::kWarps, 1) cached_kernel(const C
             codes_to_half(w1[i], a[1], a[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma_f16(s[m][n], a, q_hi[half * 4 + i][n][0], q_hi[half * 4 + i][n][1]);
-              if (kSplit) mma_f16(s[m][n], a, q_lo[half * 4 + i][n][0], q_lo[half * 4 + i][n][1]);
+              mma_f16(kSplit ? fresh[0][n] : s[m][n], a, q_hi[half * 4 + i][n][0], q_hi[half * 4 + i][n][1]);
+              if (kSplit) mma_f16(fresh[kSplit][n], a, q_lo[half * 4 + i][n][0], q_lo[half * 4 + i][n][1]);
             }
+          }
+          if (kSplit) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[m][n][i] += fresh[0][n][i] + fresh[kSplit][n][i];
           }
         }
       }
@@ -472,6 +480,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::kWarps, 1) cached_kernel(const C
         const uint4 first = *reinterpret_cast<const uint4*>(tile + ((16 * d + octet) << c.token_bits));
         const uint4 second = *reinterpret_cast<const uint4*>(tile + ((16 * d + octet + 8) << c.token_bits));
         const uint32_t w0[4] = {first.x, first.y, first.z, first.w}, w1[4] = {second.x, second.y, second.z, second.w};
+        float fresh[kSplit ? 2 : 1][NT][4] = {};
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           uint32_t a[4];
@@ -479,9 +488,15 @@ __global__ void __launch_bounds__(32 * Ring<D>::kWarps, 1) cached_kernel(const C
           codes_to_half(w1[m], a[1], a[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            mma_f16(o[d][n], a, p_hi[m][n][0], p_hi[m][n][1]);
-            if (kSplit) mma_f16(o[d][n], a, p_lo[m][n][0], p_lo[m][n][1]);
+            mma_f16(kSplit ? fresh[0][n] : o[d][n], a, p_hi[m][n][0], p_hi[m][n][1]);
+            if (kSplit) mma_f16(fresh[kSplit][n], a, p_lo[m][n][0], p_lo[m][n][1]);
           }
+        }
+        if (kSplit) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][n][i] += fresh[0][n][i] + fresh[kSplit][n][i];
         }
       }
     }
