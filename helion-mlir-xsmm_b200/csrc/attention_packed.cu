@@ -72,8 +72,9 @@ __device__ __forceinline__ void packed_row_again(const PackedParams& p, const T*
 // softmax in f32. Eight warps: four runs of 16 rows, two halves of each tile's keys, joined at the end. The products are
 // mma m16n8k16 on bf16 pieces: an f32 value is the sum of three (8 bits each, the exponent range of f32, so nothing
 // has to be scaled), and a product the six of their products that reach 2^-27; Q, K, V and P alike. That is f32's own
-// accuracy at six instructions; FFMA tiles of 64 x 64 stood still on shared memory at a third of FFMA's rate (five
-// sequences of 300, 6 heads of 80: 84 us; one of 4096, 8 heads of 64: 775 us). bf16 values are one piece.
+// accuracy at six instructions; FFMA tiles of 64 x 64 stood still on shared memory at a third of FFMA's rate. Five sequences of
+// 300, 6 heads of 80, f32: 60 us and 84 with FFMA; one of 4096, 8 heads of 64: 547 and 775. What bounds it: mma.sync, and the loads
+// of a tile, which nothing covers but the other CTA of the SM. bf16 values are one piece (2048 rows, 16/4 heads of 80: 201 us).
 constexpr int kTile = 64, kMmaThreads = 256;
 
 template <typename T, int DP>
@@ -428,7 +429,8 @@ void launch_mma_any(const PackedParams& p, cudaStream_t s) {
 // under the power cap (0.71 and 0.75 of measured cuBLAS). Measured and not kept there: P in columns of its own with blocks
 // of 80 keys, which ends the waiting but costs more softmax and MMA time a key (519 against 482 us); 16 softmax warps, two to a
 // row (496); taking turns at the exponentials (506); the maximum taken alongside stale exponentials (519); a cubic
-// for 0, 1/4 or 3/8 of the exponentials in place of 1/8 (491, 482, 530 against 468).
+// for 0, 1/4 or 3/8 of the exponentials in place of 1/8 (491, 482, 530 against 468); a CTA that goes on to further tiles, taken
+// back from the launch hardware (503 against 471: the loop costs the softmax more than the saved set-up gives).
 // Masks cost only the blocks that they cut.
 constexpr int kQRows = 128, kKeys = 128;
 constexpr int kUmmaThreads = 384, kUmmaProducerWarp = 8, kUmmaMmaWarp = 9;

@@ -463,8 +463,9 @@ int b200_symm_open(const void* handle /* B200_IPC_HANDLE_BYTES */, void** out_pt
 int b200_symm_close(void* ptr);
 int b200_symm_free(void* ptr);
 
-/* Device error word written by kernels whose bounded waits ran out
- * (0 = none). Reading it synchronises the given stream. */
+/* Device error word written by kernels whose bounded waits ran out, or that met bad
+ * offsets (256) or bad block numbers (512) (0 = none; 1024: a wait of b200_attention_cached,
+ * 2048: one of b200_attention_packed). Reading it synchronises the given stream. */
 int b200_read_kernel_status(void* stream, int32_t* out_status);
 
 /* Self-test of the failure path of the kernels' bounded waits (no counterpart in
