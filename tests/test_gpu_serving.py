@@ -182,6 +182,19 @@ def test_packed_unseen_values_may_be_huge(ops) -> None:
         within(out, want[:140], bound[:140], f"huge {dtype}")
 
 
+def test_packed_queries_that_are_not_finite(ops) -> None:
+    """A query with a NaN or an infinity answers NaN; the rows beside it in its tile do not notice."""
+    for dtype, dim in ((BF16, 128), (F32, 64), (BF16, 40)):
+        q, k, v = packed_operands(dtype, dim, 2, 1, 200, 200, 6)
+        want, bound = ref.attention_packed(q, k, v, [0, 200], [0, 200], dim ** -0.5, True, p_step(dtype))
+        q[70, 1, 3], q[130, 0, 0] = NAN, INF
+        out = ops.attention_packed(q.cuda(), k.cuda(), v.cuda(), ints([0, 200])).cpu()
+        hit = torch.zeros(200, 2, dtype=torch.bool)
+        hit[70, 1] = hit[130, 0] = True
+        assert out[hit].isnan().all()
+        within(out[~hit], want[~hit], bound[~hit], f"{dtype} {dim}")
+
+
 def test_packed_rows_behind_the_last_sequence(ops) -> None:
     for dtype, dim in ((BF16, 128), (F32, 64)):
         q, k, v = packed_operands(dtype, dim, 3, 1, 500, 500, 2)
@@ -304,6 +317,21 @@ def test_append(ops, dtype, dim: int, tokens: int) -> None:
     check_append(ops, dtype, 3, dim, tokens, [1, 0, tokens - 1, 9], [1, 1, 1, 1], use_offsets=False)
     check_append(ops, dtype, 3, dim, tokens, [1, 0, tokens - 1], [3, 3, 3], use_offsets=False)
     check_append(ops, dtype, 1, dim, tokens, [11] * 40, [1 + i % 3 for i in range(40)], x_scale=4.0, seed=7)  # scales grow
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_append_uneven_and_padded(ops, dtype) -> None:
+    """One long prompt among sequences that get nothing (few tokens on average), and rows of no sequence."""
+    check_append(ops, dtype, 2, 128, 16, [3] * 30, [0] * 17 + [90] + [0] * 12)
+    check_append(ops, dtype, 2, 64, 64, [60, 1, 64], [9, 0, 2], x_scale=0.01)
+    cache = ops.quantized_cache(4, 2, 64, 16)
+    x = torch.randn(50, 2, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[20:] = NAN  # padding behind the last sequence
+    ops.cache_append(cache, x.cuda(), x.cuda(), ints([[0, 1], [2, 3]]), ints([0, 0]), ints([0, 5, 20]))
+    assert torch.isfinite(cache.k_scales).all() and torch.isfinite(cache.v_scales).all()
+    k, _ = ops.cache_read(cache, ints([[0, 1], [2, 3]]), ints([0, 0]), ints([5, 15]), ints([0, 5, 20]), 20, F32)
+    step = x[:20].abs().amax().item() / 127
+    assert (k.cpu() - x[:20].float()).abs().max() <= 0.5 * step * 1.001
 
 
 def test_append_ties_zeros_and_extremes(ops) -> None:
@@ -442,6 +470,27 @@ def test_cached_long(ops) -> None:
     check_cached(ops, BF16, 128, 4, 1, 64, [20000], seed=1)
     check_cached(ops, F32, 64, 2, 1, 16, [7001], seed=2)
     check_cached(ops, BF16, 64, 2, 1, 32, [6000, 10, 0, 333, 2500, 1] * 2, seed=3)
+
+
+def test_blocks_beyond_32_bits(ops) -> None:
+    """Codes of the last blocks of a cache of 5 GB: offsets pass 2^31."""
+    heads, dim, tokens, blocks, lengths = 8, 128, 64, 40000, [150]
+    cache = ops.quantized_cache(blocks, heads, dim, tokens)
+    assert cache.k_codes.numel() > 2 ** 31
+    table = torch.tensor([[blocks - 1, 7, blocks - 2]], dtype=torch.int32)
+    small = ops.quantized_cache(3, heads, dim, tokens)
+    near = torch.tensor([[0, 1, 2]], dtype=torch.int32)
+    x = torch.randn(2, 150, heads, dim, generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    q = torch.randn(1, 16, dim, generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    answers = []
+    for c, t in ((cache, table), (small, near)):
+        ops.cache_append(c, x[0, :149], x[1, :149], t.cuda(), ints([0]), ints([0, 149]))
+        ops.cache_append(c, x[0, 149:], x[1, 149:], t.cuda(), ints([149]))
+        answers.append((ops.attention_cached(q, c, t.cuda(), ints(lengths)),
+                        *ops.cache_read(c, t.cuda(), ints([0]), ints(lengths), ints([0, 150]), 150)))
+    for far, close in zip(*answers):
+        assert torch.equal(far, close)
+    assert torch.equal(cache.v_codes[blocks - 1], small.v_codes[0])
 
 
 def test_cached_growing_scores_and_uneven_scales(ops) -> None:
