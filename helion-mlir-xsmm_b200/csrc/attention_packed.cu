@@ -511,6 +511,28 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 32 * kUmmaProducerWarp) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&bars->q_full[t]), 1);
+      mbar_init(smem_u32(&bars->s_full[t]), 1);
+      mbar_init(smem_u32(&bars->p_full[t][0]), 4);
+      mbar_init(smem_u32(&bars->p_full[t][1]), 4);
+      mbar_init(smem_u32(&bars->o_done[t]), 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(smem_u32(&bars->k_full[s]), 1);
+      mbar_init(smem_u32(&bars->k_empty[s]), 1);
+      mbar_init(smem_u32(&bars->v_full[s]), 1);
+      mbar_init(smem_u32(&bars->v_empty[s]), 1);
+    }
+    bars->abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  __syncwarp();
+
   // Which piece: the last rows of a sequence, which see the most keys, come first.
   const int rows_each = u.head_pairs ? kQRows : 2 * kQRows;
   const int64_t pieces = gridDim.x / u.pairs;
@@ -551,26 +573,34 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
   const int most = max(blocks[0], blocks[1]);
   const int kv_head = head[0] / p.group;
 
-  if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(smem_u32(&bars->q_full[t]), 1);
-      mbar_init(smem_u32(&bars->s_full[t]), 1);
-      mbar_init(smem_u32(&bars->p_full[t][0]), 4);
-      mbar_init(smem_u32(&bars->p_full[t][1]), 4);
-      mbar_init(smem_u32(&bars->o_done[t]), 1);
+  // The first copies are on their way before tensor memory is allocated and the warps meet.
+  const int key_begin = static_cast<int>(theirs.begin), ready = min(kStages, most);
+  auto load_keys = [&](int j, uint32_t stage) {  // lane 0: block j of K, lane 1: of V
+    const uint32_t full = smem_u32(lane == 0 ? &bars->k_full[stage] : &bars->v_full[stage]);
+    mbar_expect_tx(full, kTileBytes);
+    if (lane == 0) {
+      for (int c = 0; c < kChunks; ++c)
+        tma_load_3d(k_smem + stage * kTileBytes + c * 16384, &map_k, full, 64 * c, key_begin + j * kKeys, kv_head);
+    } else {
+      for (int h = 0; h < 2; ++h)
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d(v_smem + stage * kTileBytes + h * kVHalfBytes + c * 8192, &map_v, full, 64 * c,
+                      key_begin + j * kKeys + 64 * h, kv_head);
     }
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(smem_u32(&bars->k_full[s]), 1);
-      mbar_init(smem_u32(&bars->k_empty[s]), 1);
-      mbar_init(smem_u32(&bars->v_full[s]), 1);
-      mbar_init(smem_u32(&bars->v_empty[s]), 1);
+  };
+  if (warp == kUmmaProducerWarp && lane < 2) {
+    if (lane == 0) {
+      for (int t = 0; t < 2; ++t) {
+        if (!blocks[t]) continue;
+        const uint32_t qf = smem_u32(&bars->q_full[t]);
+        mbar_expect_tx(qf, kTileBytes);
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d(q_smem + t * kTileBytes + c * 16384, &map_q, qf, 64 * c, static_cast<int>(mine.begin + row0[t]), head[t]);
+      }
     }
-    bars->abort_flag = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&map_q);
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
+    for (int j = 0; j < ready; ++j) load_keys(j, j);
   }
+  __syncwarp();
   if (warp == kUmmaMmaWarp) {
     tmem_alloc<1>(smem_u32(&bars->tmem_base), 512);
     tmem_relinquish<1>();
@@ -583,33 +613,13 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
   if (warp >= 8) {
     // 384 threads x 168 registers at launch = 128 x (2 x 208 + 88)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    const int key_begin = static_cast<int>(theirs.begin);
     if (warp == kUmmaProducerWarp && lane < 2) {
       // ---------------------------------------------------------------- TMA producers
-      if (lane == 0) {
-        for (int t = 0; t < 2; ++t) {
-          if (!blocks[t]) continue;
-          const uint32_t qf = smem_u32(&bars->q_full[t]);
-          mbar_expect_tx(qf, kTileBytes);
-          for (int c = 0; c < kChunks; ++c)
-            tma_load_3d(q_smem + t * kTileBytes + c * 16384, &map_q, qf, 64 * c, static_cast<int>(mine.begin + row0[t]), head[t]);
-        }
-      }
-      uint32_t stage = 0, parity = 1;  // a fresh barrier's preceding phase counts as complete
-      for (int j = 0; j < most; ++j) {
-        const uint32_t empty = smem_u32(lane == 0 ? &bars->k_empty[stage] : &bars->v_empty[stage]);
-        const uint32_t full = smem_u32(lane == 0 ? &bars->k_full[stage] : &bars->v_full[stage]);
-        if (!mbar_wait(empty, parity, abort_flag, p.status, kErrPackedWait)) break;
-        mbar_expect_tx(full, kTileBytes);
-        if (lane == 0) {
-          for (int c = 0; c < kChunks; ++c)
-            tma_load_3d(k_smem + stage * kTileBytes + c * 16384, &map_k, full, 64 * c, key_begin + j * kKeys, kv_head);
-        } else {
-          for (int h = 0; h < 2; ++h)
-            for (int c = 0; c < kChunks; ++c)
-              tma_load_3d(v_smem + stage * kTileBytes + h * kVHalfBytes + c * 8192, &map_v, full, 64 * c,
-                          key_begin + j * kKeys + 64 * h, kv_head);
-        }
+      uint32_t stage = 0, parity = 0;
+      for (int j = ready; j < most; ++j) {
+        if (!mbar_wait(smem_u32(lane == 0 ? &bars->k_empty[stage] : &bars->v_empty[stage]), parity, abort_flag, p.status, kErrPackedWait))
+          break;
+        load_keys(j, stage);
         if (++stage == kStages) {
           stage = 0;
           parity ^= 1u;
