@@ -425,8 +425,8 @@ void launch_mma_any(const PackedParams& p, cudaStream_t s) {
 // special-function unit (16 a cycle and SM: 1024 cycles a block, as long as the two products). What bounds it now is
 // that softmax: of the 3210 cycles of a period a group works 1950 (maximum 250, exponentials 1420, the rest loads, stores
 // and signals: one warp to a scheduler hides little of its own latencies) and waits 1250 for the products, which the other
-// group's work covers only in part. One sequence of 8192, 32/8 heads of 128: 1174 TFLOP/s in short runs, 1045 sustained
-// under the power cap (0.71 and 0.75 of measured cuBLAS). Measured and not kept there: P in columns of its own with blocks
+// group's work covers only in part. One sequence of 8192, 32/8 heads of 128: 463 us, 1187 TFLOP/s in short runs, 1058 sustained
+// under the power cap (0.72 and 0.76 of measured cuBLAS); 4099 tokens in nine sequences 54 us; eight prompts of 128 12.6 us. Measured and not kept there: P in columns of its own with blocks
 // of 80 keys, which ends the waiting but costs more softmax and MMA time a key (519 against 482 us); 16 softmax warps, two to a
 // row (496); taking turns at the exponentials (506); the maximum taken alongside stale exponentials (519); a cubic
 // for 0, 1/4 or 3/8 of the exponentials in place of 1/8 (491, 482, 530 against 468); a CTA that goes on to further tiles, taken
@@ -809,10 +809,13 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
         }
         if (row < my_rows) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v8[8] = {o[8 * i],     o[8 * i + 1], o[8 * i + 2], o[8 * i + 3],
-                                 o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]};
-            *reinterpret_cast<uint4*>(dst + c * 32 + 8 * i) = pack16(v8);
+          for (int i = 0; i < 2; ++i) {  // whole sectors: 32 bytes a thread (in 16: 14.6 in place of 12.6 us for eight prompts of 128)
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(o[16 * i + 2 * e], o[16 * i + 2 * e + 1]);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 32 + 16 * i), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
           }
         }
       }
@@ -856,7 +859,7 @@ bool tma_strides(const void* base, int64_t row, int64_t head) {
 bool umma_takes(const b200_packed_attention_desc& d) {
   return d.dtype == B200_BF16 && (d.dim == 64 || d.dim == 128) && d.scale > 0.f && d.rows_k > 0 &&
          tma_strides(d.q, d.q_row, d.q_head) && tma_strides(d.k, d.k_row, d.k_head) && tma_strides(d.v, d.v_row, d.v_head) &&
-         aligned(d.out, 16);
+         aligned(d.out, 32);
 }
 
 template <int D>
