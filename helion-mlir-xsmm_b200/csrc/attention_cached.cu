@@ -5,8 +5,8 @@
 // sees nothing is zeros. No reference counterpart.
 //
 // Bound by HBM (measured: 4 sequences of up to 131072, 64/8 heads of 128, 107 us, 6.1 TB/s, 0.94 of measured copy bandwidth; 64 of up
-// to 4096, 32/8 heads, 57 us, 5.8 TB/s; one of 777, 8/2 heads of 64, 7.8 us, latency): every code is read once, 2 dim bytes a token and key/value head, against
-// 4 dim flops a token and query head. Each warp is a worker of its own: all tiles of 64 positions of all
+// to 4096, 32/8 heads, 57 us, 5.8 TB/s; one of 777, 8/2 heads of 64, 7.8 us, latency): every code is read once,
+// 2 dim bytes a token and key/value head, against 4 dim flops a token and query head. Each warp is a worker of its own: all tiles of 64 positions of all
 // (sequence, key/value head) pairs are numbered in one line, and worker w takes the w-th equal part of it, so
 // ragged lengths leave nobody idle, whatever they are (the host never reads them). A pair that lies
 // in one part is finished there; of the others each worker leaves its maximum, sum and

@@ -447,6 +447,11 @@ def raw_stream(index: int) -> int:
     return _raw_stream(index)
 
 
+def empty_like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of ``t``'s shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def index_of(*tensors: torch.Tensor | None) -> int:
     """The index of the CUDA device that all operands are on, for calls that are made often (a tenth of the time of
     :func:`require_cuda`, whose errors it raises)."""

@@ -103,28 +103,34 @@ _DTYPES = {torch.float32: native.F32, torch.bfloat16: native.BF16}
 
 def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor) -> int:
     """The element type's code, after the checks of the operands."""
-    shape, k_shape = q.shape, k.shape
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    shape, k_shape, code = q.shape, k.shape, _DTYPES.get(q.dtype)
+    if len(shape) != 3 or len(k_shape) != 3 or v.dim() != 3:
         raise ValueError(f"attention_packed() expects [rows, heads, dim] operands, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k_shape != v.shape or k_shape[2] != shape[2] or k_shape[1] == 0 or shape[1] == 0 or shape[1] % k_shape[1]:
+    rows, heads, dim = shape
+    key_rows, kv_heads, key_dim = k_shape
+    if k_shape != v.shape or key_dim != dim or kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError("attention_packed() operands do not match (the heads of q have to be a multiple of those of k and v): "
                          f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if not 1 <= shape[2] <= _MAX_DIM:
+    if not 1 <= dim <= _MAX_DIM:
         raise ValueError(f"attention_packed() expects heads of 1 to {_MAX_DIM}, got {tuple(q.shape)}")
-    code = _DTYPES.get(q.dtype)
     if code is None or not q.dtype is k.dtype is v.dtype:
         raise ValueError(f"attention_packed() requires matching bf16/f32 operands, got {q.dtype}, {k.dtype}, {v.dtype}")
-    for name, t in (("offsets", offsets), ("k_offsets", k_offsets)):
-        if t.dtype is not torch.int32 or t.dim() != 1 or t.shape != offsets.shape or t.shape[0] < 1 or not t.is_contiguous():
-            raise ValueError(f"attention_packed() expects {name} as a contiguous int32 tensor [sequences + 1], got {t.dtype} {tuple(t.shape)}")
-    if k_offsets is offsets and k_shape[0] != shape[0]:
+    _check_offsets("offsets", offsets, offsets)
+    if k_offsets is not offsets:
+        _check_offsets("k_offsets", k_offsets, offsets)
+    elif key_rows != rows:
         raise ValueError(f"attention_packed() needs k_offsets where k has other rows than q: {tuple(q.shape)}, {tuple(k.shape)}")
     return code
 
 
-def _tensor_core(q: Tensor, scale: float) -> bool:
+def _check_offsets(name: str, t: Tensor, like: Tensor) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or len(t) != len(like) or len(t) == 0 or not t.is_contiguous():
+        raise ValueError(f"attention_packed() expects {name} as a contiguous int32 tensor [sequences + 1], got {t.dtype} {tuple(t.shape)}")
+
+
+def _tensor_core(dtype: torch.dtype, dim: int, scale: float) -> bool:
     """Whether the tcgen05 kernel takes these operands (else mma tiles of any head size)."""
-    return q.dtype is torch.bfloat16 and q.shape[2] in _FUSED_DIMS and scale > 0.0
+    return dtype is torch.bfloat16 and dim in _FUSED_DIMS and scale > 0.0
 
 
 def _for_tma(t: Tensor) -> Tensor:
@@ -149,21 +155,24 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
 
     The offsets are not read on the host: a captured call can be replayed with other lengths of the same total. Offsets
     that decrease or leave the tensors raise bit 256 of ``native.kernel_status()`` and leave their rows unwritten."""
-    k_offsets = offsets if k_offsets is None else k_offsets
+    if k_offsets is None:
+        k_offsets = offsets
     code = _check_packed(q, k, v, offsets, k_offsets)
     index = native.index_of(q, k, v, offsets, k_offsets)
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    rows, heads, dim = q.shape
+    key_rows, kv_heads, _ = k.shape
+    scale = dim ** -0.5 if scale is None else float(scale)
     with native.on_index(index):
-        if _tensor_core(q, scale):
+        if _tensor_core(q.dtype, dim, scale):
             q, k, v = _for_tma(q), _for_tma(k), _for_tma(v)
-        else:
-            q, k, v = (t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous() for t in (q, k, v))
-        rows, heads, dim = q.shape
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif dim > 1:
+            q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+        out = native.empty_like(q)
+        (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
         result = native.module().b200_attention_packed(
-            _PACK_PACKED(code, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *q.stride()[:2],
-                         *k.stride()[:2], *v.stride()[:2], rows, k.shape[0], offsets.shape[0] - 1, heads, k.shape[1], dim,
-                         offsets.data_ptr(), k_offsets.data_ptr(), scale, 0),
+            _PACK_PACKED(code, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_row, q_head, k_row, k_head,
+                         v_row, v_head, rows, key_rows, len(offsets) - 1, heads, kv_heads, dim, offsets.data_ptr(),
+                         k_offsets.data_ptr(), scale, 0),
             native.raw_stream(index))
     native.check("b200_attention_packed", result)
     return out
@@ -172,7 +181,7 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
 def _explain_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: Tensor | None = None,
                     scale: float | None = None, causal: bool = True) -> CallExplanation:
     _check_packed(q, k, v, offsets, offsets if k_offsets is None else k_offsets)
-    if _tensor_core(q, 1.0 if scale is None else scale):
+    if _tensor_core(q.dtype, q.shape[2], 1.0 if scale is None else scale):
         return CallExplanation(True, "packed_umma_kernel (tcgen05, two tiles of 128 queries x 128 keys per step, scores in TMEM)")
     return CallExplanation(True, "packed_mma_kernel (mma bf16, f32 values in three pieces, 64 queries a CTA)")
 

@@ -23,7 +23,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 from typing import NamedTuple
 
 import torch
@@ -68,10 +67,11 @@ _DTYPES = {torch.float32: native.F32, torch.bfloat16: native.BF16}
 def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[int, ...]:
     """The fields of ``b200_kv_cache``, after the checks of the four tensors."""
     k_codes, v_codes, k_scales, v_scales = cache
-    if k_codes.dim() != 4:
+    shape = k_codes.shape
+    if len(shape) != 4:
         raise ValueError(f"{name}() expects codes [blocks, heads, tokens, dim] and [blocks, heads, dim, tokens], "
                          f"got {tuple(k_codes.shape)} and {tuple(v_codes.shape)}")
-    blocks, heads, tokens, dim = k_codes.shape
+    blocks, heads, tokens, dim = shape
     if dim not in HEAD_DIMS or tokens not in BLOCK_TOKENS or heads < 1:
         raise ValueError(f"{name}() expects blocks of {BLOCK_TOKENS} tokens and heads of {HEAD_DIMS}, got codes {tuple(k_codes.shape)}")
     if v_codes.shape != (blocks, heads, dim, tokens) or k_scales.shape != (blocks, heads) or v_scales.shape != (blocks, heads):
@@ -86,18 +86,19 @@ def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[
 
 def _indices(name: str, what: str, t: Tensor, count: int) -> int:
     """The address of an int32 vector of ``count`` values."""
-    if t.dtype is not torch.int32 or t.shape != (count,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != 1 or len(t) != count or not t.is_contiguous():
         raise ValueError(f"{name}() expects {what} as a contiguous int32 tensor [{count}], got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _table(name: str, table: Tensor) -> tuple[int, int, int]:
     """Sequences, row stride and width of a block table."""
-    if table.dtype is not torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"{name}() expects block_table as an int32 tensor [sequences, blocks] with contiguous rows, "
-                         f"got {table.dtype} {tuple(table.shape)}")
+    if table.dtype is not torch.int32 or table.dim() != 2:
+        raise ValueError(f"{name}() expects block_table as an int32 tensor [sequences, blocks], got {table.dtype} {tuple(table.shape)}")
     batch, width = table.shape
-    stride = table.stride(0)
+    stride, step = table.stride()
+    if width > 1 and step != 1:
+        raise ValueError(f"{name}() expects block_table with contiguous rows, got strides {table.stride()}")
     if batch > 1 and stride < width:
         raise ValueError(f"{name}() expects block_table rows that do not overlap, got strides {table.stride()}")
     return batch, stride, width
@@ -130,21 +131,24 @@ def cache_append(cache: tuple[Tensor, Tensor, Tensor, Tensor], k: Tensor, v: Ten
     code = _DTYPES.get(k.dtype)
     if code is None or k.dtype is not v.dtype or k.shape != v.shape:
         raise ValueError(f"cache_append() expects matching bf16/f32 k and v, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    if k.dim() == 4 and offsets is None and k.shape[0] == batch:
+    shape = k.shape
+    if len(shape) == 4 and offsets is None and shape[0] == batch:
         k, v = k.flatten(0, 1), v.flatten(0, 1)
-    elif k.dim() != 3 or (offsets is None and k.shape[0] != batch):
+        shape = k.shape
+    elif len(shape) != 3 or (offsets is None and shape[0] != batch):
         raise ValueError(f"cache_append() expects k and v [rows, heads, dim] with offsets, or [sequences, heads, dim] or [sequences, new, "
                          f"heads, dim] of {batch} sequences without, got {tuple(k.shape)}")
-    if k.shape[1] != heads or k.shape[2] != dim:
+    if shape[1] != heads or shape[2] != dim:
         raise ValueError(f"cache_append() expects k and v of {heads} heads of {dim}, got {tuple(k.shape)}")
     lengths_ptr = _indices("cache_append", "lengths", lengths, batch)
     offsets_ptr = 0 if offsets is None else _indices("cache_append", "offsets", offsets, batch + 1)
     index = native.index_of(k, v, *cache, block_table, lengths, offsets)
     with native.on_index(index):
         k, v = _aligned_rows(k), _aligned_rows(v)
+        (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
         result = native.module().b200_kv_append(
-            _PACK_APPEND(*fields, code, 0, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                         block_table.data_ptr(), lengths_ptr, offsets_ptr, stride, width, batch, k.shape[0]),
+            _PACK_APPEND(*fields, code, 0, k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, block_table.data_ptr(),
+                         lengths_ptr, offsets_ptr, stride, width, batch, shape[0]),
             native.raw_stream(index))
     native.check("b200_kv_append", result)
 
@@ -175,13 +179,13 @@ def cache_read(cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor
 
 def _check_cached(q: Tensor, heads: int, dim: int, batch: int) -> tuple[int, int, int]:
     """Element type, tokens and query heads."""
-    code, rank = _DTYPES.get(q.dtype), q.dim()
-    if code is None or rank not in (3, 4) or q.shape[-1] != dim or q.shape[-2] % heads:
+    code, shape = _DTYPES.get(q.dtype), q.shape
+    if code is None or len(shape) not in (3, 4) or shape[-1] != dim or shape[-2] % heads:
         raise ValueError(f"attention_cached() expects bf16/f32 q [sequences, heads, {dim}] or [sequences, tokens, heads, {dim}] with "
                          f"heads a multiple of {heads}, got {q.dtype} {tuple(q.shape)}")
-    if q.shape[0] != batch or q.shape[-2] == 0:
+    if shape[0] != batch or shape[-2] == 0:
         raise ValueError(f"attention_cached() expects q of {batch} sequences and at least one head, got {tuple(q.shape)}")
-    return code, 1 if rank == 3 else q.shape[1], q.shape[-2]
+    return code, 1 if len(shape) == 3 else shape[1], shape[-2]
 
 
 @functools.lru_cache(maxsize=1024)
@@ -209,12 +213,13 @@ def attention_cached(q: Tensor, cache: tuple[Tensor, Tensor, Tensor, Tensor], bl
     with native.on_index(index):
         if q.stride(-1) != 1:
             q = q.contiguous()
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = native.empty_like(q)
+        steps = q.stride()
         need = _workspace_bytes(index, fields[5], dim, fields[7], width, batch, tokens, heads)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         result = native.module().b200_attention_cached(
-            _PACK_CACHED(*fields, code, 1.0 / math.sqrt(dim) if scale is None else scale, q.data_ptr(), out.data_ptr(), q.stride(0),
-                         q.stride(1) if tokens > 1 else 0, q.stride(-2), block_table.data_ptr(), lengths_ptr, stride, width, batch,
+            _PACK_CACHED(*fields, code, dim ** -0.5 if scale is None else scale, q.data_ptr(), out.data_ptr(), steps[0],
+                         steps[1] if tokens > 1 else 0, steps[-2], block_table.data_ptr(), lengths_ptr, stride, width, batch,
                          tokens, heads, workspace.data_ptr(), need),
             native.raw_stream(index))
     native.check("b200_attention_cached", result)
