@@ -124,7 +124,7 @@ def _check_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets: T
 
 
 def _check_offsets(name: str, t: Tensor, like: Tensor) -> None:
-    if t.dtype is not torch.int32 or t.dim() != 1 or len(t) != len(like) or len(t) == 0 or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != like.numel() or t.numel() == 0 or not t.is_contiguous():
         raise ValueError(f"attention_packed() expects {name} as a contiguous int32 tensor [sequences + 1], got {t.dtype} {tuple(t.shape)}")
 
 
@@ -171,7 +171,7 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, k_offsets
         (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
         result = native.module().b200_attention_packed(
             _PACK_PACKED(code, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_row, q_head, k_row, k_head,
-                         v_row, v_head, rows, key_rows, len(offsets) - 1, heads, kv_heads, dim, offsets.data_ptr(),
+                         v_row, v_head, rows, key_rows, offsets.numel() - 1, heads, kv_heads, dim, offsets.data_ptr(),
                          k_offsets.data_ptr(), scale, 0),
             native.raw_stream(index))
     native.check("b200_attention_packed", result)

@@ -86,7 +86,7 @@ def _describe(cache: tuple[Tensor, Tensor, Tensor, Tensor], name: str) -> tuple[
 
 def _indices(name: str, what: str, t: Tensor, count: int) -> int:
     """The address of an int32 vector of ``count`` values."""
-    if t.dtype is not torch.int32 or t.dim() != 1 or len(t) != count or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
         raise ValueError(f"{name}() expects {what} as a contiguous int32 tensor [{count}], got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -168,7 +168,8 @@ def cache_read(cache: tuple[Tensor, Tensor, Tensor, Tensor], block_table: Tensor
     offsets_ptr = _indices("cache_read", "offsets", offsets, batch + 1)
     index = native.index_of(*cache, block_table, starts, lengths, offsets)
     with native.on_index(index):
-        k, v = torch.empty((2, rows, heads, dim), dtype=dtype, device=block_table.device).unbind(0)
+        k = torch.empty(rows, heads, dim, dtype=dtype, device=block_table.device)
+        v = torch.empty_like(k)
         result = native.module().b200_kv_read(
             _PACK_READ(*fields, code, 0, k.data_ptr(), v.data_ptr(), block_table.data_ptr(), starts_ptr, lengths_ptr, offsets_ptr,
                        stride, width, batch, rows),
